@@ -17,6 +17,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhga_b200.so")
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+E4M3_CODE = 3    # torch.float8_e4m3fn, the 8-bit operands of hga_fp8_linear
 
 _lib = None
 _lock = threading.Lock()
@@ -72,6 +73,14 @@ _SIGNATURES = {
                                               _I64, _P, _P, _I32, _P, _I32, _P]),
     "hga_append_tokens": (ctypes.c_int, [ctypes.POINTER(HgaParams), _I32, _P, _P, _P, _P, _P, _P, _I64, _I32, _P, _P,
                                          _I64, _P, _P]),
+    "hga_fp8_quantize": (ctypes.c_int, [_I64, _I64, _I32, _P, _I64, _P, _I64, _P, _P]),
+    "hga_fp8_linear_workspace": (ctypes.c_int64, [_I64, _I64, _I64, _I32, _P, _I64, _P, _I64]),
+    "hga_fp8_linear": (ctypes.c_int, [_I64, _I64, _I64, _I32, _P, _I64, _P, _P, _I64, _P, _I64, _P, _I32, _P, _I64, _P,
+                                      _I64, _P]),
+    "hga_kv4_pack": (ctypes.c_int, [_I32, _I32, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _P]),
+    "hga_kv4_unpack": (ctypes.c_int, [_I32, _I32, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _P]),
+    "hga_attend_decode_kv4": (ctypes.c_int, [ctypes.POINTER(HgaParams), _I32, _P, _P, _P, _P, _I64, _P, _P, _I64, _P,
+                                             _P, _I32, _P, _P]),
     "hga_device_status": (ctypes.c_int, [_P, _I32]),
     "hga_qkv_prologue": (ctypes.c_int, [ctypes.POINTER(HgaParams), _I64, _P, _I64, _P, _P, ctypes.c_float, _I32, _P,
                                         _P, _I32, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _P]),
@@ -146,7 +155,7 @@ def make_params(*, batch, nhead, kv_heads, head_dim, chunk_size, group_size, top
 
 def device_status(clear: bool = True) -> int:
     """First device error code of the kernels (0 = none): a bounded tensor-core wait that timed out,
-    or a decode bounds check (0x101 routing, 0x102 attention, 0x103 append)."""
+    or a decode bounds check (0x101 routing, 0x102 attention, 0x103 append, 0x104 4-bit attention)."""
     code = ctypes.c_int32(0)
     check(lib().hga_device_status(ctypes.byref(code), 1 if clear else 0), "hga_device_status")
     return int(code.value)

@@ -3,6 +3,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include "fp8_common.cuh"
 #include "hga_common.cuh"
 
 namespace hga {
@@ -72,6 +73,18 @@ cudaError_t launch_attend_decode_fast(const hga_params& p, int L, const void* q,
 cudaError_t launch_append(const hga_params& p, int L, const int32_t* seq_pos, const void* kr, const void* v,
                           const void* kraw, void* hk, void* hv, int64_t hot_cap, int hot_mode, void* ck, void* cv,
                           int64_t cold_cap, void* act_raw, cudaStream_t st);
+cudaError_t launch_fp8_quantize(int dtype, const void* x, int64_t x_stride, int64_t m, int64_t k, void* q,
+                                int64_t q_stride, int64_t q_cols, float* scale, cudaStream_t st);
+int64_t fp8_linear_workspace(const Fp8Linear& a);
+cudaError_t launch_fp8_linear(const Fp8Linear& a, cudaStream_t st);
+cudaError_t launch_kv4_pack(int dtype, int dh, int64_t heads, int64_t rows, const void* k, const void* v, int64_t cap,
+                            void* rec_k, void* rec_v, int64_t unit_cap, int64_t unit0, cudaStream_t st);
+cudaError_t launch_kv4_unpack(int dtype, int dh, int64_t heads, int64_t rows, const void* rec_k, const void* rec_v,
+                              int64_t unit_cap, int64_t unit0, void* k, void* v, int64_t cap, cudaStream_t st);
+cudaError_t launch_attend_kv4(const hga_params& p, int L, const void* q, const int32_t* seq_pos, const void* hk,
+                              const void* hv, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
+                              const int32_t* og, const int32_t* ot, int Kg, void* out, cudaStream_t st);
+int kv4_error_status(bool clear);
 }  // namespace hga
 
 static thread_local char g_err[512];
@@ -441,6 +454,101 @@ int hga_shard_unpack(const void* recv, int64_t rank_stride, int64_t part_offset,
                      "hga_shard_unpack");
 }
 
+int hga_fp8_quantize(int64_t m, int64_t k, int32_t dtype, const void* x, int64_t x_stride, void* q, int64_t q_stride,
+                     float* scale, cudaStream_t stream) {
+  if (m < 0 || k <= 0) return fail(HGA_E_INVALID, "hga_fp8_quantize: need m >= 0 and k > 0");
+  if (dtype < HGA_DTYPE_F32 || dtype > HGA_DTYPE_F16) return fail(HGA_E_INVALID, "hga_fp8_quantize: unknown dtype %d", dtype);
+  if (m == 0) return HGA_OK;
+  if (!x || !q || !scale) return fail(HGA_E_INVALID, "hga_fp8_quantize: NULL tensor");
+  if (x_stride < k || q_stride < k) return fail(HGA_E_INVALID, "hga_fp8_quantize: row stride smaller than the row");
+  return cuda_status(hga::launch_fp8_quantize(dtype, x, x_stride, m, k, q, q_stride, k, scale, stream),
+                     "hga_fp8_quantize");
+}
+
+int64_t hga_fp8_linear_workspace(int64_t m, int64_t n, int64_t k, int32_t x_dtype, const void* x, int64_t x_stride,
+                                 const void* w, int64_t w_stride) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  hga::Fp8Linear a{};
+  a.m = m; a.n = n; a.k = k;
+  a.x_dtype = x_dtype; a.x = x; a.x_stride = x_stride; a.w = w; a.w_stride = w_stride;
+  return hga::fp8_linear_workspace(a);
+}
+
+int hga_fp8_linear(int64_t m, int64_t n, int64_t k, int32_t x_dtype, const void* x, int64_t x_stride,
+                   const float* x_scale, const void* w, int64_t w_stride, const float* w_scale, int64_t ws_stride,
+                   const void* bias, int32_t out_dtype, void* out, int64_t out_stride, void* workspace,
+                   int64_t workspace_bytes, cudaStream_t stream) {
+  if (m < 0 || n <= 0 || k <= 0) return fail(HGA_E_INVALID, "hga_fp8_linear: need m >= 0, n > 0 and k > 0");
+  if (m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffff00) return fail(HGA_E_UNSUPPORTED, "hga_fp8_linear: a size is over 2^31");
+  if (x_dtype < HGA_DTYPE_F32 || x_dtype > HGA_DTYPE_E4M3) return fail(HGA_E_INVALID, "hga_fp8_linear: unknown x_dtype %d", x_dtype);
+  if (out_dtype < HGA_DTYPE_F32 || out_dtype > HGA_DTYPE_F16)
+    return fail(HGA_E_INVALID, "hga_fp8_linear: unknown out_dtype %d", out_dtype);
+  if (m == 0) return HGA_OK;
+  if (!x || !w || !w_scale || !out) return fail(HGA_E_INVALID, "hga_fp8_linear: NULL tensor");
+  if (x_dtype == HGA_DTYPE_E4M3 && !x_scale) return fail(HGA_E_INVALID, "hga_fp8_linear: 8-bit x needs x_scale");
+  if (x_stride < k || w_stride < k || out_stride < n || ws_stride < (k + 127) / 128)
+    return fail(HGA_E_INVALID, "hga_fp8_linear: row stride smaller than the row");
+  const hga::Fp8Linear a{m, n, k, x, x_stride, x_dtype, x_scale, w, w_stride, w_scale, ws_stride, bias, out, out_stride,
+                         out_dtype, workspace};
+  const int64_t need = hga::fp8_linear_workspace(a);
+  if (need > workspace_bytes || (need && (!workspace || ((uintptr_t)workspace & 15))))
+    return fail(HGA_E_INVALID, "hga_fp8_linear: needs %lld bytes of 16-byte aligned workspace", (long long)need);
+  return cuda_status(hga::launch_fp8_linear(a, stream), "hga_fp8_linear");
+}
+
+static int check_kv4(const char* what, int32_t dtype, int32_t head_dim, int64_t heads, int64_t rows, const void* k,
+                     const void* v, int64_t kv_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
+                     int64_t unit0) {
+  if (dtype < HGA_DTYPE_F32 || dtype > HGA_DTYPE_F16) return fail(HGA_E_INVALID, "%s: unknown dtype %d", what, dtype);
+  if (head_dim <= 0 || head_dim % 64 || head_dim > 256)
+    return fail(HGA_E_UNSUPPORTED, "%s: head_dim must be 64, 128, 192 or 256", what);
+  if (heads < 0 || rows < 0) return fail(HGA_E_INVALID, "%s: negative size", what);
+  if (heads == 0 || rows == 0) return HGA_OK;
+  if (!k || !v || !rec_k || !rec_v) return fail(HGA_E_INVALID, "%s: NULL tensor", what);
+  if (kv_cap < rows) return fail(HGA_E_INVALID, "%s: kv_cap < rows", what);
+  if (unit0 < 0 || unit0 + (rows + 15) / 16 > unit_cap) return fail(HGA_E_INVALID, "%s: record capacity too small", what);
+  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)rec_k | (uintptr_t)rec_v) & 15)
+    return fail(HGA_E_INVALID, "%s: pointers must be 16-byte aligned", what);
+  return HGA_OK;
+}
+
+int hga_kv4_pack(int32_t dtype, int32_t head_dim, int64_t heads, int64_t rows, const void* k, const void* v,
+                 int64_t kv_cap, void* rec_k, void* rec_v, int64_t unit_cap, int64_t unit0, cudaStream_t stream) {
+  const int rc = check_kv4("hga_kv4_pack", dtype, head_dim, heads, rows, k, v, kv_cap, rec_k, rec_v, unit_cap, unit0);
+  if (rc || heads == 0 || rows == 0) return rc;
+  return cuda_status(hga::launch_kv4_pack(dtype, head_dim, heads, rows, k, v, kv_cap, rec_k, rec_v, unit_cap, unit0,
+                                          stream),
+                     "hga_kv4_pack");
+}
+
+int hga_kv4_unpack(int32_t dtype, int32_t head_dim, int64_t heads, int64_t rows, const void* rec_k, const void* rec_v,
+                   int64_t unit_cap, int64_t unit0, void* k, void* v, int64_t kv_cap, cudaStream_t stream) {
+  const int rc = check_kv4("hga_kv4_unpack", dtype, head_dim, heads, rows, k, v, kv_cap, rec_k, rec_v, unit_cap, unit0);
+  if (rc || heads == 0 || rows == 0) return rc;
+  return cuda_status(hga::launch_kv4_unpack(dtype, head_dim, heads, rows, rec_k, rec_v, unit_cap, unit0, k, v, kv_cap,
+                                            stream),
+                     "hga_kv4_unpack");
+}
+
+int hga_attend_decode_kv4(const hga_params* p, int32_t L, const void* q, const int32_t* seq_pos, const void* hot_k,
+                          const void* hot_v, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
+                          const int32_t* open_gid, const int32_t* open_t0, int32_t Kg, void* out, cudaStream_t stream) {
+  int rc = check_params(p);
+  if (rc) return rc;
+  if (L <= 0 || L > p->chunk_size) return fail(HGA_E_INVALID, "hga_attend_decode_kv4: 1 <= L <= chunk_size");
+  if (p->head_dim % 64) return fail(HGA_E_UNSUPPORTED, "hga_attend_decode_kv4: head_dim must be 64, 128, 192 or 256");
+  if (p->group_size % 16) return fail(HGA_E_UNSUPPORTED, "hga_attend_decode_kv4: group_size must be a multiple of 16");
+  if (Kg < 0 || unit_cap < 0) return fail(HGA_E_INVALID, "hga_attend_decode_kv4: negative size");
+  if (!q || !seq_pos || !hot_k || !hot_v || !out) return fail(HGA_E_INVALID, "hga_attend_decode_kv4: NULL tensor");
+  if (Kg > 0 && (!open_gid || !open_t0 || !rec_k || !rec_v))
+    return fail(HGA_E_INVALID, "hga_attend_decode_kv4: NULL open lists / record");
+  if (((uintptr_t)q | (uintptr_t)hot_k | (uintptr_t)hot_v | (uintptr_t)out | (uintptr_t)rec_k | (uintptr_t)rec_v) & 15)
+    return fail(HGA_E_INVALID, "hga_attend_decode_kv4: pointers must be 16-byte aligned");
+  return cuda_status(hga::launch_attend_kv4(*p, L, q, seq_pos, hot_k, hot_v, hot_cap, rec_k, rec_v, unit_cap, open_gid,
+                                            open_t0, Kg, out, stream),
+                     "hga_attend_decode_kv4");
+}
+
 int hga_debug_fault(int32_t mode, int64_t wait_limit_ns) {
   if (mode < 0 || mode > 1 || wait_limit_ns < 0) return fail(HGA_E_INVALID, "hga_debug_fault: mode 0/1, wait_limit_ns >= 0");
   hga::attend_tc_set_test_fault(mode, (long long)wait_limit_ns);
@@ -448,8 +556,9 @@ int hga_debug_fault(int32_t mode, int64_t wait_limit_ns) {
 }
 
 int hga_device_status(int32_t* code, int32_t clear) {
-  const int words[4] = {hga::tc_error_status(clear != 0), hga::route_tc_error_status(clear != 0),
-                        hga::decode_error_status(clear != 0), hga::decode_fast_error_status(clear != 0)};
+  const int words[5] = {hga::tc_error_status(clear != 0), hga::route_tc_error_status(clear != 0),
+                        hga::decode_error_status(clear != 0), hga::decode_fast_error_status(clear != 0),
+                        hga::kv4_error_status(clear != 0)};
   int first = 0;
   for (int w : words) {
     if (w < 0) return fail(HGA_E_CUDA, "hga_device_status: cannot read the device error word");

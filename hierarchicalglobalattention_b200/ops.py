@@ -375,6 +375,225 @@ def append_tokens(p: HgaParams, seq_pos: torch.Tensor, k_rope: torch.Tensor, v: 
                                   stream_ptr(k_rope.device)), "hga_append_tokens")
 
 
+# ---------------------------------------------------------------------------------------------
+# 8-bit block-scaled products
+# ---------------------------------------------------------------------------------------------
+FP8_BLOCK = 128
+_FP8_X = {**_lib.DTYPE_CODE, torch.float8_e4m3fn: _lib.E4M3_CODE}
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [..., K] as [M, K] rows with unit stride in the last dimension (a view where one exists)."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [..., K] (fp32 / bf16 / fp16) as e4m3 values [..., K] and fp32 scales [..., ceil(K / 128)], one
+    per row and block of 128 channels (see hga_fp8_quantize)."""
+    _require_cuda(x)
+    code = _lib.DTYPE_CODE.get(x.dtype)
+    if code is None or x.dim() == 0 or x.shape[-1] == 0:
+        raise _lib.HgaError(f"fp8_quantize takes fp32 / bf16 / fp16 rows of at least one channel; got {x.dtype} "
+                            f"{tuple(x.shape)}")
+    K = x.shape[-1]
+    r = _rows(x)
+    M = r.shape[0]
+    q = torch.empty(*x.shape[:-1], K, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(*x.shape[:-1], -(-K // FP8_BLOCK), device=x.device, dtype=torch.float32)
+    check(lib().hga_fp8_quantize(M, K, code, r.data_ptr(), max(r.stride(0), K), q.data_ptr(), K, scale.data_ptr(),
+                                 stream_ptr(x.device)), "hga_fp8_quantize")
+    return q, scale
+
+
+def fp8_quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A weight [N, K] as e4m3 values and one fp32 scale per 128 x 128 block (amax / 448; 1 for a block of
+    zeros), [ceil(N / 128), ceil(K / 128)]: the format of block-scaled 8-bit checkpoints.  Runs once when
+    a layer is loaded, on any device."""
+    if w.dim() != 2 or w.numel() == 0:
+        raise _lib.HgaError(f"fp8_quantize_weight takes a non-empty [N, K] weight; got {tuple(w.shape)}")
+    N, K = w.shape
+    nb, kb = -(-N // FP8_BLOCK), -(-K // FP8_BLOCK)
+    p = torch.zeros(nb * FP8_BLOCK, kb * FP8_BLOCK, device=w.device, dtype=torch.float32)
+    p[:N, :K] = w
+    blocks = p.view(nb, FP8_BLOCK, kb, FP8_BLOCK)
+    amax = blocks.abs().amax(dim=(1, 3))
+    scale = torch.where(amax <= 1e-30, torch.ones_like(amax), amax / 448.0)
+    q = (blocks / scale[:, None, :, None]).reshape(nb * FP8_BLOCK, kb * FP8_BLOCK)[:N, :K]
+    return q.to(torch.float8_e4m3fn).contiguous(), scale.contiguous()
+
+
+def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               x_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = x w^T (+ bias) with an e4m3 weight w [N, K] and fp32 scales w_scale [ceil(N / 128),
+    ceil(K / 128)] (see hga_fp8_linear).  x [..., K]: fp32 / bf16 / fp16 rows are quantised per row and
+    128 channels on the way in; e4m3 rows come with ``x_scale`` [..., ceil(K / 128)], as fp8_quantize
+    returns them.  The result [..., N] has ``out_dtype``: x's type, or bf16 for 8-bit x.  ``bias`` [N] has
+    the result's type."""
+    _require_cuda(x, w, w_scale, bias, x_scale)
+    code = _FP8_X.get(x.dtype)
+    if code is None:
+        raise _lib.HgaError(f"fp8_linear: x must be fp32, bf16, fp16 or e4m3; got {x.dtype}")
+    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.stride(1) != 1:
+        raise _lib.HgaError("fp8_linear: w must be an e4m3 [N, K] tensor with contiguous rows")
+    N, K = w.shape
+    KB = -(-K // FP8_BLOCK)
+    if x.dim() == 0 or x.shape[-1] != K or K == 0 or N == 0:
+        raise _lib.HgaError(f"fp8_linear: x {tuple(x.shape)} does not fit w {tuple(w.shape)}")
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != (-(-N // FP8_BLOCK), KB) or w_scale.stride(1) != 1:
+        raise _lib.HgaError(f"fp8_linear: w_scale must be fp32 [{-(-N // FP8_BLOCK)}, {KB}] with contiguous rows")
+    xs = None
+    if code == _lib.E4M3_CODE:
+        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (*x.shape[:-1], KB):
+            raise _lib.HgaError("fp8_linear: 8-bit x needs x_scale, fp32 [..., ceil(K / 128)]")
+        xs = x_scale.contiguous()
+        out_dtype = out_dtype or torch.bfloat16
+    elif x_scale is not None:
+        raise _lib.HgaError("fp8_linear: x_scale goes with 8-bit x only")
+    out_dtype = out_dtype or x.dtype
+    ocode = _lib.DTYPE_CODE.get(out_dtype)
+    if ocode is None:
+        raise _lib.HgaError(f"fp8_linear: out_dtype must be fp32, bf16 or fp16; got {out_dtype}")
+    if bias is not None and (bias.dtype != out_dtype or bias.shape != (N,) or not bias.is_contiguous()):
+        raise _lib.HgaError(f"fp8_linear: bias must be a contiguous [{N}] tensor of the result's type")
+    dev = x.device
+    for t in (w, w_scale, bias, xs, out):
+        if t is not None and t.device != dev:
+            raise _lib.HgaError("fp8_linear: tensors on different devices")
+    r = _rows(x)
+    M = r.shape[0]
+    if out is None:
+        out = torch.empty(*x.shape[:-1], N, device=dev, dtype=out_dtype)
+    elif out.dtype != out_dtype or out.shape != (*x.shape[:-1], N) or not out.is_contiguous():
+        raise _lib.HgaError("fp8_linear: out must be a contiguous [..., N] tensor of the result's type")
+    h = lib()
+    xp, wp, xst, wst = r.data_ptr(), w.data_ptr(), max(r.stride(0), K), max(w.stride(0), K)
+    need = h.hga_fp8_linear_workspace(M, N, K, code, xp, xst, wp, wst)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    check(h.hga_fp8_linear(M, N, K, code, xp, xst, ptr(xs), wp, wst, w_scale.data_ptr(), max(w_scale.stride(0), KB),
+                           ptr(bias), ocode, out.data_ptr(), N, ptr(ws), need, stream_ptr(dev)), "hga_fp8_linear")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
+# 4-bit KV record
+# ---------------------------------------------------------------------------------------------
+KV4_UNIT = 16
+
+
+def kv4_unit_bytes(head_dim: int) -> int:
+    """Bytes of one 16-token unit of K (or V) in the 4-bit record."""
+    return 10 * head_dim
+
+
+def _kv4_rec(name: str, rec: torch.Tensor, B: int, KVH: int, Dh: int) -> int:
+    """Units allocated per (sequence, KV head) of a record [B, KVH, units, 10 * Dh]."""
+    if (rec.dtype != torch.uint8 or rec.dim() != 4 or rec.shape[0] != B or rec.shape[1] != KVH
+            or rec.shape[3] != 10 * Dh or not rec.is_contiguous()):
+        raise _lib.HgaError(f"{name}: a record is a contiguous uint8 [B, KVH, units, 10 * Dh] tensor; got {rec.dtype} "
+                            f"{tuple(rec.shape)} for B={B}, KVH={KVH}, Dh={Dh}")
+    if rec.device.type != "cuda" and not rec.is_pinned():
+        raise _lib.HgaError(f"{name}: a record in host memory must be pinned")
+    return rec.shape[2]
+
+
+def _kv4_rows(t: torch.Tensor) -> torch.Tensor:
+    """K/V rows as a row-slice of a contiguous [B,KVH,cap,Dh] buffer (copied when they are laid out otherwise)."""
+    B, KVH, S, Dh = t.shape
+    ok = (t.stride(3) == 1 and t.stride(2) == Dh and t.stride(1) % Dh == 0 and t.stride(1) >= S * Dh
+          and t.stride(0) == KVH * t.stride(1) and t.data_ptr() % 16 == 0)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+             unit0: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Token rows k / v [B,KVH,S,Dh] into units [unit0, unit0 + ceil(S / 16)) of a 4-bit record ``rec`` =
+    (rec_k, rec_v), uint8 [B,KVH,units,10*Dh] on the device or in pinned host memory; a new device record
+    of just these rows when None (see hga_kv4_pack).  Returns the record."""
+    _require_cuda(k, v)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _lib.DTYPE_CODE:
+        raise _lib.HgaError("kv4_pack: k and v must be [B,KVH,S,Dh] tensors of one shape and type (fp32 / bf16 / fp16)")
+    B, KVH, S, Dh = k.shape
+    units = -(-S // KV4_UNIT)
+    if rec is None:
+        rec_k = torch.empty(B, KVH, unit0 + units, 10 * Dh, device=k.device, dtype=torch.uint8)
+        rec_v = torch.empty_like(rec_k)
+    else:
+        rec_k, rec_v = rec
+    cap = _kv4_rec("kv4_pack", rec_k, B, KVH, Dh)
+    if _kv4_rec("kv4_pack", rec_v, B, KVH, Dh) != cap:
+        raise _lib.HgaError("kv4_pack: rec_k and rec_v differ in capacity")
+    if k.numel() == 0:
+        return rec_k, rec_v
+    k, v = _kv4_rows(k), _kv4_rows(v)
+    if k.stride(1) != v.stride(1):
+        k, v = k.contiguous(), v.contiguous()
+    check(lib().hga_kv4_pack(_lib.DTYPE_CODE[k.dtype], Dh, B * KVH, S, k.data_ptr(), v.data_ptr(), k.stride(1) // Dh,
+                             rec_k.data_ptr(), rec_v.data_ptr(), cap, unit0, stream_ptr(k.device)), "hga_kv4_pack")
+    return rec_k, rec_v
+
+
+def kv4_unpack(rec_k: torch.Tensor, rec_v: torch.Tensor, seq_len: int, dtype: torch.dtype, unit0: int = 0,
+               device: Optional[torch.device] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values of ``seq_len`` rows from unit ``unit0`` on: k, v [B,KVH,seq_len,Dh] in ``dtype``, the type
+    that was packed (see hga_kv4_unpack).  ``device``: where to, for a record in pinned host memory."""
+    if dtype not in _lib.DTYPE_CODE:
+        raise _lib.HgaError(f"kv4_unpack: dtype must be fp32, bf16 or fp16; got {dtype}")
+    if rec_k.dim() != 4 or rec_k.shape[3] % 10:
+        raise _lib.HgaError("kv4_unpack: a record is a uint8 [B, KVH, units, 10 * Dh] tensor")
+    B, KVH, _, nb = rec_k.shape
+    Dh = nb // 10
+    cap = _kv4_rec("kv4_unpack", rec_k, B, KVH, Dh)
+    if _kv4_rec("kv4_unpack", rec_v, B, KVH, Dh) != cap:
+        raise _lib.HgaError("kv4_unpack: rec_k and rec_v differ in capacity")
+    dev = rec_k.device if device is None else torch.device(device)
+    if dev.type != "cuda":
+        raise _lib.HgaError("hga ops run on CUDA tensors only (no CPU fallback): give kv4_unpack a CUDA device")
+    k = torch.empty(B, KVH, seq_len, Dh, device=dev, dtype=dtype)
+    v = torch.empty_like(k)
+    check(lib().hga_kv4_unpack(_lib.DTYPE_CODE[dtype], Dh, B * KVH, seq_len, rec_k.data_ptr(), rec_v.data_ptr(), cap,
+                               unit0, k.data_ptr(), v.data_ptr(), seq_len, stream_ptr(dev)), "hga_kv4_unpack")
+    return k, v
+
+
+def attend_decode_kv4(p: HgaParams, q: torch.Tensor, seq_pos: torch.Tensor, hot_k: torch.Tensor, hot_v: torch.Tensor,
+                      rec_k: torch.Tensor, rec_v: torch.Tensor, open_gid: torch.Tensor, open_t0: torch.Tensor,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one decode block q [B,H,L,Dh] over the slot windows hot_* (hot_mode 1's layout) and the
+    opened groups of a 4-bit record (see hga_attend_decode_kv4).  Returns [B,H,L,Dh]."""
+    _require_cuda(q, seq_pos, hot_k, hot_v, open_gid, open_t0)
+    if not q.is_contiguous():
+        q = q.contiguous()
+    B, H, L, Dh = q.shape
+    if (B, H, Dh) != (p.batch, p.nhead, p.head_dim) or _lib.DTYPE_CODE.get(q.dtype) != p.dtype:
+        raise _lib.HgaError(f"attend_decode_kv4: q {tuple(q.shape)} {q.dtype} does not fit the layer's parameters")
+    if hot_k.dtype != q.dtype or hot_v.dtype != q.dtype or hot_k.shape != hot_v.shape:
+        raise _lib.HgaError("attend_decode_kv4: hot_k / hot_v must have q's type and one shape")
+    if (seq_pos.dtype != torch.int32 or open_gid.dtype != torch.int32 or open_t0.dtype != torch.int32
+            or seq_pos.numel() != B or open_gid.shape != open_t0.shape or tuple(open_gid.shape[:2]) != (B, H)):
+        raise _lib.HgaError("attend_decode_kv4: seq_pos [B] and open_gid / open_t0 [B,H,Kg] must be int32")
+    if not open_gid.is_contiguous() or not open_t0.is_contiguous():
+        open_gid, open_t0 = open_gid.contiguous(), open_t0.contiguous()
+    KVH = p.kv_heads
+    cap = _kv4_rec("attend_decode_kv4", rec_k, B, KVH, Dh)
+    if _kv4_rec("attend_decode_kv4", rec_v, B, KVH, Dh) != cap:
+        raise _lib.HgaError("attend_decode_kv4: rec_k and rec_v differ in capacity")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise _lib.HgaError("attend_decode_kv4: out must be contiguous, of q's shape and type")
+    hot_cap = kv_cap_of(hot_k)
+    if kv_cap_of(hot_v) != hot_cap:
+        raise _lib.HgaError("attend_decode_kv4: hot_k and hot_v must share one capacity layout")
+    check(lib().hga_attend_decode_kv4(ctypes_params(p), L, q.data_ptr(), seq_pos.data_ptr(), hot_k.data_ptr(),
+                                      hot_v.data_ptr(), hot_cap, rec_k.data_ptr(), rec_v.data_ptr(), cap,
+                                      open_gid.data_ptr(), open_t0.data_ptr(), open_gid.shape[2], out.data_ptr(),
+                                      stream_ptr(q.device)), "hga_attend_decode_kv4")
+    return out
+
+
 def shard_unpack(recv: torch.Tensor, rank_stride: int, part_offset: int, world: int, pieces: int,
                  dst_block, bk: int, rows: int, row_bytes: int, dst: torch.Tensor) -> None:
     """Scatter one part of an all-gathered multi-GPU prefill buffer into sequence order (see

@@ -26,7 +26,8 @@
 extern "C" {
 #endif
 
-enum { HGA_DTYPE_F32 = 0, HGA_DTYPE_BF16 = 1, HGA_DTYPE_F16 = 2 };
+enum { HGA_DTYPE_F32 = 0, HGA_DTYPE_BF16 = 1, HGA_DTYPE_F16 = 2,
+       HGA_DTYPE_E4M3 = 3 /* 8-bit operands of hga_fp8_linear only */ };
 /* How hga_summaries reads its rotary table. */
 enum { HGA_ROT_F32 = 0,         /* fp32 table, used as fp32 (ChunkRouter._rotary_for_positions) */
        HGA_ROT_MODEL = 1,       /* table already in the model dtype */
@@ -251,9 +252,60 @@ int hga_shard_unpack(const void* recv, int64_t rank_stride, int64_t part_offset,
                      const int32_t* dst_block, int64_t bk, int64_t rows, int64_t row_bytes, void* dst,
                      cudaStream_t stream);
 
+/* ---- 8-bit block-scaled products (no counterpart in the reference, whose FP8 checkpoints go through
+ * the model library's own layers: "FP8-safe" patch, qwen_routed_attention.py:94-156) --------------
+ *
+ * hga_fp8_quantize: rows x [m][k] (F32, BF16 or F16; row stride x_stride elements) to e4m3 with one
+ * fp32 scale per row and block of 128 channels (the last block may be short):
+ *   scale = amax / 448 (1 where amax <= 1e-30),  q = e4m3(x / scale), nearest, ties to even.
+ * q [m][k] with row stride q_stride bytes; scale [m][ceil(k / 128)].  A block that holds an infinity
+ * or a NaN gets a non-finite scale (its products are NaN). */
+int hga_fp8_quantize(int64_t m, int64_t k, int32_t dtype, const void* x, int64_t x_stride, void* q, int64_t q_stride,
+                     float* scale, cudaStream_t stream);
+
+/* hga_fp8_linear: y = x w^T (+ bias) with w [n][k] in e4m3 (row stride w_stride bytes) and one fp32 scale
+ * per 128 x 128 block, w_scale [ceil(n / 128)][>= ceil(k / 128)] (row stride ws_stride elements):
+ *   y[m][n] = sum_kb x_scale[m][kb] * w_scale[n / 128][kb] * sum_{k in kb} xq[m][k] * w[n][k] + bias[n].
+ * x_dtype F32 / BF16 / F16: x is quantised as hga_fp8_quantize does; E4M3: x and x_scale
+ * [m][ceil(k / 128)] are used as they are (x_scale is ignored otherwise).  Products and sums in fp32,
+ * one rounding to out_dtype (F32 / BF16 / F16) at the end; bias [n] in out_dtype, or NULL.  x_stride and
+ * out_stride in elements, any value >= the row.  The call needs hga_fp8_linear_workspace(...) bytes of
+ * 16-byte aligned device memory, which it may overwrite (0 bytes: workspace may be NULL). */
+int64_t hga_fp8_linear_workspace(int64_t m, int64_t n, int64_t k, int32_t x_dtype, const void* x, int64_t x_stride,
+                                 const void* w, int64_t w_stride);
+int hga_fp8_linear(int64_t m, int64_t n, int64_t k, int32_t x_dtype, const void* x, int64_t x_stride,
+                   const float* x_scale, const void* w, int64_t w_stride, const float* w_scale, int64_t ws_stride,
+                   const void* bias, int32_t out_dtype, void* out, int64_t out_stride, void* workspace,
+                   int64_t workspace_bytes, cudaStream_t stream);
+
+/* ---- 4-bit KV record (no counterpart in the reference, whose records hold the model dtype) -----------
+ * Token rows of K and V in units of 16 rows per (sequence, KV head): 4-bit codes with a 16-bit scale and
+ * minimum per token and 32 channels, 10 * head_dim bytes a unit instead of 32 * head_dim (BF16).  With
+ * lo, hi the extremes of a token's block: min = lo, scale = (hi - lo) * fp32(1 / 15), each rounded to the cache's
+ * type (BF16 for an F32 cache); code = clamp(rint((x - min) / scale), 0, 15), 0 where scale is 0; the
+ * value read back is scale * code + min (fp32, then rounded to the type).  A block with an infinity or
+ * a NaN reads back as NaN.  Byte layout: csrc/kv4_common.cuh.  head_dim must be 64, 128, 192 or 256.
+ *
+ * hga_kv4_pack: rows [0, rows) of k / v [heads][kv_cap][head_dim] into units [unit0, unit0 + ceil(rows / 16))
+ * of rec_k / rec_v [heads][unit_cap][10 * head_dim] (heads = batch * kv_heads; missing rows of the last
+ * unit read back as 0).  hga_kv4_unpack: the inverse.  The record may be device memory or pinned host
+ * memory; every pointer 16-byte aligned. */
+int hga_kv4_pack(int32_t dtype, int32_t head_dim, int64_t heads, int64_t rows, const void* k, const void* v,
+                 int64_t kv_cap, void* rec_k, void* rec_v, int64_t unit_cap, int64_t unit0, cudaStream_t stream);
+int hga_kv4_unpack(int32_t dtype, int32_t head_dim, int64_t heads, int64_t rows, const void* rec_k, const void* rec_v,
+                   int64_t unit_cap, int64_t unit0, void* k, void* v, int64_t kv_cap, cudaStream_t stream);
+
+/* hga_attend_decode_kv4: hga_attend_decode with hot_mode 1 whose opened groups come from a 4-bit record
+ * (unit g * (group_size / 16) is the first unit of group g; group_size a multiple of 16, rec_* device or
+ * pinned host memory).  Windows and the active chunk are read from the slots in the cache's type.  Rows of the
+ * slots and the record that a query row does not see do not count, whatever they hold. */
+int hga_attend_decode_kv4(const hga_params* p, int32_t L, const void* q, const int32_t* seq_pos, const void* hot_k,
+                          const void* hot_v, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
+                          const int32_t* open_gid, const int32_t* open_t0, int32_t Kg, void* out, cudaStream_t stream);
+
 /* Device-side error words: 0, or the first code recorded.  The tensor-core kernels record a
  * bounded mbarrier wait that timed out (the CTA then released its TMEM and returned without
- * output); the decode kernels record 0x101 / 0x102 / 0x103 (routing / attention / append) when a
+ * output); the decode kernels record 0x101 / 0x102 / 0x103 / 0x104 (routing / attention / append / 4-bit attention) when a
  * sequence position or a list entry addresses rows past a buffer's capacity (those rows are
  * skipped; a (b, h) whose position is past the capacity gets a zero output), and 0x101 also when
  * a sequence's routed pool exceeds the nmid_max given to hga_route_decode (its lists stay -1).
