@@ -73,8 +73,6 @@ cudaError_t launch_attend_decode_fast(const hga_params& p, int L, const void* q,
 cudaError_t launch_append(const hga_params& p, int L, const int32_t* seq_pos, const void* kr, const void* v,
                           const void* kraw, void* hk, void* hv, int64_t hot_cap, int hot_mode, void* ck, void* cv,
                           int64_t cold_cap, void* act_raw, cudaStream_t st);
-cudaError_t launch_fp8_quantize(int dtype, const void* x, int64_t x_stride, int64_t m, int64_t k, void* q,
-                                int64_t q_stride, int64_t q_cols, float* scale, cudaStream_t st);
 int64_t fp8_linear_workspace(const Fp8Linear& a);
 cudaError_t launch_fp8_linear(const Fp8Linear& a, cudaStream_t st);
 cudaError_t launch_kv4_pack(int dtype, int dh, int64_t heads, int64_t rows, const void* k, const void* v, int64_t cap,
@@ -85,6 +83,8 @@ cudaError_t launch_attend_kv4(const hga_params& p, int L, const void* q, const i
                               const void* hv, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
                               const int32_t* og, const int32_t* ot, int Kg, void* out, cudaStream_t st);
 int kv4_error_status(bool clear);
+int fp8_tiles_error_status(bool clear);
+int fp8_rows_error_status(bool clear);
 }  // namespace hga
 
 static thread_local char g_err[512];
@@ -556,9 +556,10 @@ int hga_debug_fault(int32_t mode, int64_t wait_limit_ns) {
 }
 
 int hga_device_status(int32_t* code, int32_t clear) {
-  const int words[5] = {hga::tc_error_status(clear != 0), hga::route_tc_error_status(clear != 0),
+  const int words[7] = {hga::tc_error_status(clear != 0), hga::route_tc_error_status(clear != 0),
                         hga::decode_error_status(clear != 0), hga::decode_fast_error_status(clear != 0),
-                        hga::kv4_error_status(clear != 0)};
+                        hga::kv4_error_status(clear != 0), hga::fp8_tiles_error_status(clear != 0),
+                        hga::fp8_rows_error_status(clear != 0)};
   int first = 0;
   for (int w : words) {
     if (w < 0) return fail(HGA_E_CUDA, "hga_device_status: cannot read the device error word");

@@ -1,4 +1,5 @@
-// 8-bit block-scaled operators: quantisation of activations and the product with an e4m3 weight.
+// 8-bit block-scaled operators: quantisation of activations, and the dispatch of the product with an e4m3
+// weight (its kernels are in fp8_tiles.cu, for many rows, and fp8_rows.cu, for few).
 //
 //   scale[m][kb] = max |x[m][k]|, k in block kb of 128, / 448        (1 where that maximum is <= 1e-30)
 //   q[m][k]      = e4m3(x[m][k] / scale[m][k / 128])                  round to nearest, ties to even
@@ -7,40 +8,9 @@
 // The division is the IEEE one: a reciprocal's last-bit error would move values that lie on a rounding
 // boundary of e4m3 (about one in a thousand: quotients of two bf16 numbers meet the boundaries exactly).
 // A block that holds an infinity or a NaN gets a non-finite scale, so its products are NaN.
-#include <cuda_fp8.h>
-
 #include "fp8_common.cuh"
 
 namespace hga {
-
-// largest magnitude as an integer of the float's bits without its sign: NaN is larger than infinity,
-// which is larger than every finite value, so a NaN is never lost
-__device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) {
-  const float amax = __uint_as_float(amax_bits);
-  return amax <= 1e-30f ? 1.0f : __fdiv_rn(amax, 448.0f);  // NaN compares false: the scale is NaN
-}
-
-__device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Num<T>::to_f(h[i]);
-  }
-}
 
 // One block of 128 channels of one row per 16 lanes, 8 channels a lane.  Bound by HBM: 2 bytes read
 // and 1 written per 16-bit channel.  VEC: rows and base are 16-byte aligned (8-byte for q).
@@ -71,24 +41,17 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
           if (c0 + e < k) f[e] = Num<T>::to_f(src[e]);
       }
     }
-    uint32_t a = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a = max(a, mag_bits(f[e]));
-#pragma unroll
-    for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    uint2 v;
+    const float s = fp8_block(f, v);
     if (!live) continue;
-    const float s = fp8_scale(a);
     if (lane16 == 0) scale[i] = s;
-    uint16_t h[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = e4m3x2(__fdiv_rn(f[2 * e], s), __fdiv_rn(f[2 * e + 1], s));
     uint8_t* dst = q + row * q_stride + c0;
     if (VEC && c0 + 8 <= q_cols) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+      *reinterpret_cast<uint2*>(dst) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (c0 + e < q_cols) dst[e] = (uint8_t)(h[e / 2] >> (8 * (e & 1)));
+        if (c0 + e < q_cols) dst[e] = (uint8_t)((e < 4 ? v.x : v.y) >> (8 * (e & 3)));
     }
   }
 }
@@ -122,91 +85,82 @@ cudaError_t launch_fp8_quantize(int dtype, const void* x, int64_t x_stride, int6
   return cudaErrorInvalidValue;
 }
 
-// ---- product ------------------------------------------------------------------------------------
-__device__ __forceinline__ float e4m3_f(uint8_t v) {
-  __nv_fp8_e4m3 h;
-  h.__x = v;
-  return (float)h;
-}
-
-// 64 tokens x 64 output features per CTA, one block of 128 channels at a time through shared memory,
-// 4 x 4 outputs a thread.
-template <typename T>
-__global__ void __launch_bounds__(256) fp8_product_kernel(const uint8_t* __restrict__ q, int64_t q_stride,
-                                                          const float* __restrict__ xs, const uint8_t* __restrict__ w,
-                                                          int64_t w_stride, const float* __restrict__ ws, int64_t ws_stride,
-                                                          const T* __restrict__ bias, T* __restrict__ out,
-                                                          int64_t out_stride, int64_t m, int64_t n, int64_t k, int kb) {
-  __shared__ float sa[64][33], sb[64][33];
-  const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int b = 0; b < kb; ++b) {
-    float part[4][4] = {};
-    for (int k0 = b * 128; k0 < (b + 1) * 128; k0 += 32) {
-      for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-        const int r = i / 32, c = i % 32;
-        sa[r][c] = (m0 + r < m && k0 + c < k) ? e4m3_f(q[(m0 + r) * q_stride + k0 + c]) : 0.f;
-        sb[r][c] = (n0 + r < n && k0 + c < k) ? e4m3_f(w[(n0 + r) * w_stride + k0 + c]) : 0.f;
-      }
-      __syncthreads();
-      for (int c = 0; c < 32; ++c)
+// Rows of k bytes to rows of `cols` bytes (zeros behind k), 16-byte aligned: operands that TMA cannot
+// address where they are (a base or a row stride off the 16-byte grid).
+__global__ void __launch_bounds__(256) fp8_realign_kernel(const uint8_t* __restrict__ src, int64_t src_stride,
+                                                          int64_t rows, int64_t k, uint4* __restrict__ dst, int64_t cols) {
+  const int64_t per = cols / 16, total = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per, c = (i - r * per) * 16;
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] = fmaf(sa[ty * 4 + i][c], sb[tx + 16 * j][c], part[i][j]);
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t r = m0 + ty * 4 + i, c = n0 + tx + 16 * j;
-        if (r < m && c < n) acc[i][j] = fmaf(part[i][j], xs[r * kb + b] * ws[c / 128 * ws_stride + b], acc[i][j]);
-      }
+    for (int e = 0; e < 16; ++e)
+      if (c + e < k) w[e >> 2] |= (uint32_t)src[r * src_stride + c + e] << (8 * (e & 3));
+    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = m0 + ty * 4 + i, c = n0 + tx + 16 * j;
-      if (r < m && c < n) out[r * out_stride + c] = Num<T>::from_f(acc[i][j] + (bias ? Num<T>::to_f(bias[c]) : 0.f));
-    }
 }
 
-int64_t fp8_linear_workspace(const Fp8Linear& a) {
-  const int64_t kb = (a.k + 127) / 128;
-  return a.x_dtype == HGA_DTYPE_E4M3 ? 0 : a.m * kb * 128 + a.m * kb * 4;
-}
-
-template <typename T>
-static cudaError_t product_t(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, cudaStream_t st) {
-  const int kb = (int)((a.k + 127) / 128);
-  fp8_product_kernel<T><<<dim3((unsigned)((a.n + 63) / 64), (unsigned)((a.m + 63) / 64)), 256, 0, st>>>(
-      (const uint8_t*)q, q_stride, xs, (const uint8_t*)a.w, a.w_stride, a.w_scale, a.ws_stride, (const T*)a.bias,
-      (T*)a.out, a.out_stride, a.m, a.n, a.k, kb);
+static cudaError_t realign(const void* src, int64_t stride, int64_t rows, int64_t k, void* dst, int64_t cols,
+                           cudaStream_t st) {
+  int64_t grid = (rows * (cols / 16) + 255) / 256;
+  if (grid > 148 * 8) grid = 148 * 8;
+  fp8_realign_kernel<<<(unsigned)grid, 256, 0, st>>>((const uint8_t*)src, stride, rows, k, (uint4*)dst, cols);
   return cudaGetLastError();
 }
 
+static bool off_grid(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || (stride & 15); }
+
+// Workspace: [quantised or realigned x][its scales][realigned w], each part present only where needed.
+static void parts(const Fp8Linear& a, int64_t& xq, int64_t& xs, int64_t& w) {
+  const int64_t kb = (a.k + 127) / 128;
+  xq = xs = w = 0;
+  if (a.x_dtype != HGA_DTYPE_E4M3) {
+    if (!fp8_rows_fused(a)) {
+      xq = a.m * kb * 128;
+      xs = (a.m * kb * 4 + 15) / 16 * 16;
+    }
+  } else if (off_grid(a.x, a.x_stride)) {
+    xq = a.m * kb * 128;
+  }
+  if (off_grid(a.w, a.w_stride)) w = a.n * kb * 128;
+}
+
+int64_t fp8_linear_workspace(const Fp8Linear& a) {
+  int64_t xq, xs, w;
+  parts(a, xq, xs, w);
+  return xq + xs + w;
+}
+
 cudaError_t launch_fp8_linear(const Fp8Linear& a, cudaStream_t st) {
+  const int64_t cols = (a.k + 127) / 128 * 128;
+  int64_t xqb, xsb, wb;
+  parts(a, xqb, xsb, wb);
+  char* ws = (char*)a.workspace;
   const void* q = a.x;
   int64_t q_stride = a.x_stride;
   const float* xs = a.x_scale;
-  if (a.x_dtype != HGA_DTYPE_E4M3) {
-    const int64_t kb = (a.k + 127) / 128;
-    q_stride = kb * 128;
-    float* s = (float*)((char*)a.workspace + a.m * q_stride);
-    cudaError_t e = launch_fp8_quantize(a.x_dtype, a.x, a.x_stride, a.m, a.k, a.workspace, q_stride, q_stride, s, st);
+  const void* w = a.w;
+  int64_t w_stride = a.w_stride;
+  cudaError_t e = cudaSuccess;
+  if (xqb) {
+    q = ws;
+    q_stride = cols;
+    if (xsb) {
+      xs = (const float*)(ws + xqb);
+      e = launch_fp8_quantize(a.x_dtype, a.x, a.x_stride, a.m, a.k, ws, cols, cols, (float*)(ws + xqb), st);
+    } else {
+      e = realign(a.x, a.x_stride, a.m, a.k, ws, cols, st);
+    }
     if (e != cudaSuccess) return e;
-    q = a.workspace;
-    xs = s;
   }
-  switch (a.out_dtype) {
-    case HGA_DTYPE_F32: return product_t<float>(a, q, q_stride, xs, st);
-    case HGA_DTYPE_BF16: return product_t<__nv_bfloat16>(a, q, q_stride, xs, st);
-    case HGA_DTYPE_F16: return product_t<__half>(a, q, q_stride, xs, st);
+  if (wb) {
+    w = ws + xqb + xsb;
+    w_stride = cols;
+    e = realign(a.w, a.w_stride, a.n, a.k, ws + xqb + xsb, cols, st);
+    if (e != cudaSuccess) return e;
   }
-  return cudaErrorInvalidValue;
+  if (fp8_rows_better(a)) return launch_fp8_rows(a, q, q_stride, xs, w, w_stride, st);
+  return launch_fp8_tiles(a, q, q_stride, xs, w, w_stride, st);
 }
 
 }  // namespace hga

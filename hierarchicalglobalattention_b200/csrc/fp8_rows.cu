@@ -1,0 +1,350 @@
+// Product of few rows (a decode step's tokens) with an e4m3 weight.  The weight is what has to be read, so
+// it is the 128-row operand of the tensor cores (D^T[feature][token] = w q^T) and every SM streams a part
+// of it: a CTA takes 128 features x TN tokens x a slice of the channels, and a cluster of up to 8 CTAs
+// shares one output tile along the channels, joining the partial sums through distributed shared memory in
+// a fixed order (no atomics, no second launch).
+//   warp 0     TMA producer of the weight's (and, when x comes quantised, the tokens') 128-channel blocks
+//   warp 1     MMA issuer, TMEM owner: one group of four K = 32 steps per block into its own TMEM columns
+//   warps 2-5  FUSED: quantise the CTA's slice of x straight into the swizzled shared operand while the
+//              weight is on its way (each slice is small and comes from L2); then one feature a thread:
+//              sum[token] += D * (ws * xs[token]) per block
+// FUSED saves the quantisation's launch and its round trip through memory.
+#include <cooperative_groups.h>
+
+#include "fp8_common.cuh"
+#include "tc_common.cuh"
+
+namespace hga {
+namespace tc {
+
+namespace cg = cooperative_groups;
+
+constexpr int kRowsThreads = 192;
+constexpr int kErrFp8Rows = 0x48;
+constexpr int kMaxSlice = 16;  // channel blocks per CTA
+
+struct RowsArgs {
+  int m, n, k, kb, splits;
+  const void* x;      // FUSED: the activations
+  int64_t x_stride;
+  int x_vec;          // 16-byte loads are possible
+  const float* xs;    // not FUSED: their scales
+  const float* ws;
+  int64_t ws_stride;
+  const void* bias;
+  void* out;
+  int64_t out_stride;
+};
+
+template <int TN, bool FUSED> struct RowsSmem {
+  static constexpr int kStages = TN == 64 ? 4 : 5;
+  static constexpr int kBufs = TN == 64 ? 4 : 8;               // TMEM buffers of TN columns
+  static constexpr int kW = 128 * 128, kX = TN * 128;
+  static constexpr int kStage = kW + (FUSED ? 0 : kX);
+  static constexpr int kScale = kStages * kStage;               // [kMaxSlice][TN]
+  static constexpr int kBars = kScale + kMaxSlice * TN * 4;
+  static constexpr int kNumBars = 2 * kStages + 2 * kBufs + 2;
+  static constexpr int kMisc = kBars + kNumBars * 8;
+  static constexpr int kXs = (kMisc + 32 + 1023) / 1024 * 1024;  // FUSED: the quantised slice, as long as it is
+  static constexpr int total(int slice) { return FUSED ? kXs + slice * kX : kMisc + 32; }
+  static constexpr uint32_t kCols = kBufs * TN;                 // 128 or 256
+  static_assert(kStages * kStage >= 128 * TN * 4, "the partial sums reuse the ring");
+};
+
+template <typename TX, typename TO, int TN, bool FUSED>
+__global__ void __launch_bounds__(kRowsThreads)
+    fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const RowsArgs a) {
+  using S = RowsSmem<TN, FUSED>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  // every CTA of a cluster places its parts at the same offset (the distributed reads need that): the
+  // dynamic base is the same in all of them
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* full = bars;
+  uint64_t* empty = full + S::kStages;
+  uint64_t* d_full = empty + S::kStages;
+  uint64_t* d_empty = d_full + S::kBufs;
+  uint64_t* x_ready = d_empty + S::kBufs;
+  uint64_t* drain = x_ready + 1;
+  int* misc = reinterpret_cast<int*>(smem + S::kMisc);
+  volatile int* abort_flag = misc;
+  uint32_t* tmem_s = reinterpret_cast<uint32_t*>(misc + 1);
+  float* scale_s = reinterpret_cast<float*>(smem + S::kScale);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x, n0 = blockIdx.y * 128, t0 = blockIdx.z * TN;
+  const int kb0 = (int)((int64_t)a.kb * rank / a.splits), kb1 = (int)((int64_t)a.kb * (rank + 1) / a.splits);
+  const int nkb = kb1 - kb0;
+
+  if (tid == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < S::kBufs; ++i) {
+      mbar_init(d_full + i, 1);
+      mbar_init(d_empty + i, 4);
+    }
+    mbar_init(x_ready, 128);
+    mbar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *abort_flag = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_s)),
+                 "r"(S::kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_s;
+
+  float acc[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) acc[j] = 0.f;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (; it < nkb; ++it) {
+        const int st = it % S::kStages;
+        if (it >= S::kStages && !mbar_wait(empty + st, (it / S::kStages - 1) & 1, abort_flag, kErrFp8Rows)) break;
+        unsigned char* s = smem + st * S::kStage;
+        mbar_expect_tx(full + st, S::kStage);
+        tma_load_2d(s, &tm_w, (kb0 + it) * 128, n0, full + st);
+        if constexpr (!FUSED) tma_load_2d(s + S::kW, &tm_x, (kb0 + it) * 128, t0, full + st);
+      }
+      for (int i = it > S::kStages ? it - S::kStages : 0; i < it; ++i)
+        mbar_drain(full + i % S::kStages, (i / S::kStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t id = idesc_e4m3(TN);
+      bool ok = mbar_wait(x_ready, 0, abort_flag, kErrFp8Rows + 1);
+      for (int it = 0; it < nkb && ok; ++it) {
+        const int st = it % S::kStages, buf = it % S::kBufs;
+        if (!mbar_wait(full + st, (it / S::kStages) & 1, abort_flag, kErrFp8Rows + 2) ||
+            (it >= S::kBufs && !mbar_wait(d_empty + buf, (it / S::kBufs - 1) & 1, abort_flag, kErrFp8Rows + 3)))
+          break;
+        fence_after();
+        const uint32_t wa = smem_u32(smem + st * S::kStage);
+        const uint32_t xa = FUSED ? smem_u32(smem + S::kXs + it * S::kX) : wa + S::kW;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_ss_f8(tmem + buf * TN, sdesc(wa + k * 32, 16, 1024), sdesc(xa + k * 32, 16, 1024), id, k != 0);
+        mma_commit(empty + st);
+        mma_commit(d_full + buf);
+      }
+      mma_commit(drain);
+      mbar_drain(drain, 0);
+    }
+  } else {
+    const int e = tid - 64;  // 0..127
+    if constexpr (FUSED) {
+      // 16 lanes a block of 128 channels, 8 rows at a time; the operand's 128-byte swizzle: 16-byte piece p
+      // of row r sits at p ^ (r & 7)
+      const TX* x = static_cast<const TX*>(a.x);
+      const int sub = e & 15, row8 = e >> 4;
+      constexpr int RPT = TN / 8;
+      for (int i = 0; i < nkb; ++i) {
+        const int c0 = (kb0 + i) * 128 + sub * 8;
+        float f[RPT][8];
+#pragma unroll
+        for (int j = 0; j < RPT; ++j) {
+          const int r = row8 + 8 * j;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) f[j][c] = 0.f;
+          if (t0 + r < a.m) {
+            const TX* src = x + (int64_t)(t0 + r) * a.x_stride + c0;
+            if (a.x_vec && c0 + 8 <= a.k) {
+              load8<TX>(src, f[j]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                if (c0 + c < a.k) f[j][c] = Num<TX>::to_f(src[c]);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < RPT; ++j) {
+          const int r = row8 + 8 * j;
+          uint2 v;
+          const float s = fp8_block(f[j], v);
+          *reinterpret_cast<uint2*>(smem + S::kXs + i * S::kX + r * 128 + (((sub >> 1) ^ (r & 7)) << 4) + (sub & 1) * 8) = v;
+          if (sub == 0) scale_s[i * TN + r] = s;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    } else {
+      for (int i = e; i < nkb * TN; i += 128) {
+        const int r = t0 + i % TN;
+        scale_s[i] = r < a.m ? a.xs[(int64_t)r * a.kb + kb0 + i / TN] : 0.f;
+      }
+    }
+    mbar_arrive(x_ready);
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the scales are in shared memory
+    const int quarter = warp & 3;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const float* ws = a.ws + (int64_t)blockIdx.y * a.ws_stride + kb0;
+    for (int it = 0; it < nkb; ++it) {
+      const int buf = it % S::kBufs;
+      const float w = ws[it];
+      if (!__all_sync(0xffffffffu, mbar_wait(d_full + buf, (it / S::kBufs) & 1, abort_flag, kErrFp8Rows + 4))) break;
+      fence_after();
+      uint32_t r[TN];
+      if constexpr (TN == 16) {
+        HGA_LD16(tmem + lane_addr + buf * TN, r);
+      } else {
+#pragma unroll
+        for (int c = 0; c < TN; c += 32) {
+          uint32_t(&rr)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + c);
+          HGA_LD32(tmem + lane_addr + buf * TN + c, rr);
+        }
+      }
+      tmem_wait_ld();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_empty + buf);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[j] = fmaf(__uint_as_float(r[j]), scale_s[it * TN + j] * w, acc[j]);
+    }
+  }
+
+  const int feat = (warp >= 2 ? ((warp & 3) * 32 + lane) : 0);
+  TO* out = static_cast<TO*>(a.out);
+  const TO* bias = static_cast<const TO*>(a.bias);
+  if (a.splits == 1) {
+    if (warp >= 2 && n0 + feat < a.n) {
+      const float add = bias ? Num<TO>::to_f(bias[n0 + feat]) : 0.f;
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        if (t0 + j < a.m) out[(int64_t)(t0 + j) * a.out_stride + n0 + feat] = Num<TO>::from_f(acc[j] + add);
+    }
+  } else {
+    // the ring is free: the last block's MMAs (which read it) have completed and no load is outstanding
+    float* part = reinterpret_cast<float*>(smem);  // [TN][128]
+    __syncthreads();
+    if (warp >= 2) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) part[j * 128 + feat] = acc[j];
+    }
+    cg::cluster_group cl = cg::this_cluster();
+    __syncwarp();
+    cl.sync();
+    const int lo = TN * rank / a.splits, hi = TN * (rank + 1) / a.splits;
+    for (int i = lo * 128 + tid; i < hi * 128; i += kRowsThreads) {
+      const int j = i >> 7, f = i & 127;
+      if (t0 + j < a.m && n0 + f < a.n) {
+        float s = 0.f;
+        for (int p = 0; p < a.splits; ++p) s += *cl.map_shared_rank(part + i, p);
+        if (bias) s += Num<TO>::to_f(bias[n0 + f]);
+        out[(int64_t)(t0 + j) * a.out_stride + n0 + f] = Num<TO>::from_f(s);
+      }
+    }
+    cl.sync();  // no CTA leaves while another still reads its sums
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kCols));
+}
+
+// CTAs along the channels: enough to give every SM about two CTAs' worth of weight, at least two
+// blocks each, at most 8 (a portable cluster) and kMaxSlice blocks a CTA.
+static int rows_splits(int64_t m, int64_t n, int64_t kb, int tn) {
+  const int64_t tiles = (n + 127) / 128 * ((m + tn - 1) / tn);
+  int s = 1;
+  while (s < 8 && ((tiles * s * 2 <= 148 * 2 && kb >= 4 * s) || kb > (int64_t)s * kMaxSlice)) s *= 2;
+  return s;
+}
+
+static int rows_tn(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
+
+template <typename TX, typename TO, int TN, bool FUSED>
+static cudaError_t rows_t(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
+                          int64_t w_stride, cudaStream_t st) {
+  CUtensorMap mx, mw;
+  const cuuint64_t dw[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n}, sw[1] = {(cuuint64_t)w_stride};
+  const cuuint32_t bw[2] = {128, 128};
+  if (!make_map_typed(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, 2, dw, sw, bw, CU_TENSOR_MAP_SWIZZLE_128B))
+    return cudaErrorInvalidValue;
+  mx = mw;
+  if (!FUSED) {
+    const cuuint64_t dx[2] = {(cuuint64_t)a.k, (cuuint64_t)a.m}, sx[1] = {(cuuint64_t)q_stride};
+    const cuuint32_t bx[2] = {128, TN};
+    if (!make_map_typed(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, 2, dx, sx, bx, CU_TENSOR_MAP_SWIZZLE_128B))
+      return cudaErrorInvalidValue;
+  }
+  RowsArgs r;
+  r.m = (int)a.m; r.n = (int)a.n; r.k = (int)a.k; r.kb = (int)((a.k + 127) / 128);
+  r.splits = rows_splits(a.m, a.n, r.kb, TN);
+  r.x = a.x; r.x_stride = a.x_stride;
+  r.x_vec = ((uintptr_t)a.x & 15) == 0 && (a.x_stride * (int64_t)sizeof(TX)) % 16 == 0;
+  r.xs = xs; r.ws = a.w_scale; r.ws_stride = a.ws_stride;
+  r.bias = a.bias; r.out = a.out; r.out_stride = a.out_stride;
+  const int smem = RowsSmem<TN, FUSED>::total((r.kb + r.splits - 1) / r.splits) + 1024;
+  auto kern = fp8_rows_kernel<TX, TO, TN, FUSED>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(r.splits, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + TN - 1) / TN));
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = r.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, mw, mx, r);
+}
+
+template <typename TX, typename TO, bool FUSED>
+static cudaError_t rows_m(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
+                          int64_t w_stride, cudaStream_t st) {
+  const int tn = rows_tn(a.m);
+  if (tn == 16) return rows_t<TX, TO, 16, FUSED>(a, q, q_stride, xs, w, w_stride, st);
+  if (tn == 32) return rows_t<TX, TO, 32, FUSED>(a, q, q_stride, xs, w, w_stride, st);
+  if constexpr (!FUSED) return rows_t<TX, TO, 64, false>(a, q, q_stride, xs, w, w_stride, st);
+  return cudaErrorInvalidValue;
+}
+
+template <typename TO>
+static cudaError_t rows_o(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
+                          int64_t w_stride, cudaStream_t st) {
+  if (!fp8_rows_fused(a)) return rows_m<TO, TO, false>(a, q, q_stride, xs, w, w_stride, st);
+  switch (a.x_dtype) {
+    case HGA_DTYPE_F32: return rows_m<float, TO, true>(a, q, q_stride, xs, w, w_stride, st);
+    case HGA_DTYPE_BF16: return rows_m<__nv_bfloat16, TO, true>(a, q, q_stride, xs, w, w_stride, st);
+    case HGA_DTYPE_F16: return rows_m<__half, TO, true>(a, q, q_stride, xs, w, w_stride, st);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace tc
+
+static bool rows_fit(const Fp8Linear& a) {
+  const int64_t kb = (a.k + 127) / 128;
+  return kb <= 8 * tc::kMaxSlice && (a.n + 127) / 128 <= 65535;
+}
+
+// Rows for which streaming the weight is better than 128-row tiles.
+bool fp8_rows_better(const Fp8Linear& a) { return a.m <= 256 && rows_fit(a); }
+
+bool fp8_rows_fused(const Fp8Linear& a) { return a.x_dtype != HGA_DTYPE_E4M3 && a.m <= 32 && rows_fit(a); }
+
+cudaError_t launch_fp8_rows(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
+                            int64_t w_stride, cudaStream_t st) {
+  switch (a.out_dtype) {
+    case HGA_DTYPE_F32: return tc::rows_o<float>(a, q, q_stride, xs, w, w_stride, st);
+    case HGA_DTYPE_BF16: return tc::rows_o<__nv_bfloat16>(a, q, q_stride, xs, w, w_stride, st);
+    case HGA_DTYPE_F16: return tc::rows_o<__half>(a, q, q_stride, xs, w, w_stride, st);
+  }
+  return cudaErrorInvalidValue;
+}
+
+HGA_DEFINE_ERROR_READER(fp8_rows_error_status)
+
+}  // namespace hga
