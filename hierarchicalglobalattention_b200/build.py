@@ -9,7 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libhga_b200.so")
 SOURCES = ["abi.cu", "prologue.cu", "summaries.cu", "route_prefill.cu", "attend_simt.cu", "attend_tc.cu", "route_tc.cu", "decode.cu", "decode_fast.cu", "shard.cu", "bank.cu",
-           "fp8.cu", "fp8_tiles.cu", "fp8_rows.cu", "kv4.cu"]
+           "fp8.cu", "fp8_tiles.cu", "fp8_rows.cu", "kv4.cu", "kv4_attend.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -82,7 +82,12 @@ cudaError_t launch_kv4_unpack(int dtype, int dh, int64_t heads, int64_t rows, co
 cudaError_t launch_attend_kv4(const hga_params& p, int L, const void* q, const int32_t* seq_pos, const void* hk,
                               const void* hv, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
                               const int32_t* og, const int32_t* ot, int Kg, void* out, cudaStream_t st);
+cudaError_t launch_attend_kv4_mma(const hga_params& p, int L, const void* q, const int32_t* seq_pos, const void* hk,
+                                  const void* hv, int64_t hot_cap, const void* rec_k, const void* rec_v,
+                                  int64_t unit_cap, const int32_t* og, const int32_t* ot, int Kg, void* out,
+                                  cudaStream_t st);
 int kv4_error_status(bool clear);
+int kv4_attend_error_status(bool clear);
 int fp8_tiles_error_status(bool clear);
 int fp8_rows_error_status(bool clear);
 }  // namespace hga
@@ -544,6 +549,9 @@ int hga_attend_decode_kv4(const hga_params* p, int32_t L, const void* q, const i
     return fail(HGA_E_INVALID, "hga_attend_decode_kv4: NULL open lists / record");
   if (((uintptr_t)q | (uintptr_t)hot_k | (uintptr_t)hot_v | (uintptr_t)out | (uintptr_t)rec_k | (uintptr_t)rec_v) & 15)
     return fail(HGA_E_INVALID, "hga_attend_decode_kv4: pointers must be 16-byte aligned");
+  const cudaError_t e = hga::launch_attend_kv4_mma(*p, L, q, seq_pos, hot_k, hot_v, hot_cap, rec_k, rec_v, unit_cap,
+                                                   open_gid, open_t0, Kg, out, stream);
+  if (e != cudaErrorNotSupported) return cuda_status(e, "hga_attend_decode_kv4");
   return cuda_status(hga::launch_attend_kv4(*p, L, q, seq_pos, hot_k, hot_v, hot_cap, rec_k, rec_v, unit_cap, open_gid,
                                             open_t0, Kg, out, stream),
                      "hga_attend_decode_kv4");
@@ -556,10 +564,10 @@ int hga_debug_fault(int32_t mode, int64_t wait_limit_ns) {
 }
 
 int hga_device_status(int32_t* code, int32_t clear) {
-  const int words[7] = {hga::tc_error_status(clear != 0), hga::route_tc_error_status(clear != 0),
+  const int words[8] = {hga::tc_error_status(clear != 0), hga::route_tc_error_status(clear != 0),
                         hga::decode_error_status(clear != 0), hga::decode_fast_error_status(clear != 0),
                         hga::kv4_error_status(clear != 0), hga::fp8_tiles_error_status(clear != 0),
-                        hga::fp8_rows_error_status(clear != 0)};
+                        hga::fp8_rows_error_status(clear != 0), hga::kv4_attend_error_status(clear != 0)};
   int first = 0;
   for (int w : words) {
     if (w < 0) return fail(HGA_E_CUDA, "hga_device_status: cannot read the device error word");
