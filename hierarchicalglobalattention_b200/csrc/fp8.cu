@@ -12,46 +12,56 @@
 
 namespace hga {
 
-// One block of 128 channels of one row per 16 lanes, 8 channels a lane.  Bound by HBM: 2 bytes read
-// and 1 written per 16-bit channel.  VEC: rows and base are 16-byte aligned (8-byte for q).
+// A warp takes 8 neighbouring blocks of a row, two at a time (16 lanes a block, 8 channels a lane), their
+// four loads in flight together.  The four rounds' scales and reciprocals are worked out side by side, one
+// round a lane, and handed out by shuffles: computed per round they were a third of the instructions.
+// Bound by HBM (2 bytes read and 1 written per 16-bit channel) and nearly so by issue.  VEC: rows and base are
+// 16-byte aligned (8-byte for q).
+constexpr int kQuantWarps = 8;
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, int64_t x_stride, int64_t m,
-                                                           int64_t k, int kb, uint8_t* __restrict__ q, int64_t q_stride,
-                                                           int64_t q_cols, float* __restrict__ scale) {
-  const int lane16 = threadIdx.x & 15;
-  const int64_t nblk = m * kb;
-  const int64_t step = (int64_t)gridDim.x * (blockDim.x / 16);
-  // every lane of a warp runs the same number of rounds (the shuffles below are warp-wide)
-  const int64_t first = (int64_t)blockIdx.x * (blockDim.x / 16) + threadIdx.x / 16;
-  const int64_t first0 = (int64_t)blockIdx.x * (blockDim.x / 16) + (threadIdx.x / 32) * 2;
-  for (int64_t i0 = first0, i = first; i0 < nblk; i0 += step, i += step) {
-    const bool live = i < nblk;
-    const int64_t row = live ? i / kb : 0;
-    const int64_t c0 = (live ? i - row * kb : 0) * 128 + lane16 * 8;
-    float f[8];
+__global__ void __launch_bounds__(kQuantWarps * 32) fp8_quantize_kernel(const T* __restrict__ x, int64_t x_stride,
+                                                                        int64_t m, int64_t k, int kb, int segs,
+                                                                        uint8_t* __restrict__ q, int64_t q_stride,
+                                                                        int64_t q_cols, float* __restrict__ scale) {
+  const int lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
+  const int64_t tasks = m * segs, step = (int64_t)gridDim.x * kQuantWarps;
+  for (int64_t task = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5); task < tasks; task += step) {
+    const int64_t row = (uint64_t)task >> 32 ? task / segs : (int64_t)((uint32_t)task / (uint32_t)segs);
+    const int blk0 = (int)(task - row * segs) * 8 + half;  // of round 0
+    const T* src = x + row * x_stride + (int64_t)blk0 * 128 + sub * 8;
+    const int64_t c0 = (int64_t)blk0 * 128 + sub * 8;
+    Raw8<T> raw[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.f;
-    if (live) {
-      const T* src = x + row * x_stride + c0;
-      if (VEC && c0 + 8 <= k) {
-        load8<T>(src, f);
+    for (int r = 0; r < 4; ++r)
+      raw[r] = blk0 + 2 * r < kb ? raw_load<T>(src + r * 256, VEC, k - (c0 + r * 256)) : raw_zero<T>();
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float a = raw_amax<T>(raw[r]);
+      if ((lane & 3) == r) mine = a;
+    }
+    const float my_s = fp8_scale(mine), my_inv = __frcp_rn(my_s);
+    const bool odd = __any_sync(0xffffffffu, !(my_s < INFINITY));
+    if (sub < 4 && blk0 + 2 * sub < kb) scale[row * kb + blk0 + 2 * sub] = my_s;
+    uint8_t* dst = q + row * q_stride + c0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float s = __shfl_sync(0xffffffffu, my_s, half * 16 + r), inv = __shfl_sync(0xffffffffu, my_inv, half * 16 + r);
+      float f[8];
+      raw_floats<T>(raw[r], f);
+      uint2 v = fp8_quotients(f, s, inv);
+      if (odd) {
+        if (!(s < INFINITY)) v = fp8_divisions(f, s);
+      }
+      if (blk0 + 2 * r >= kb) continue;
+      if (VEC && c0 + r * 256 + 8 <= q_cols) {
+        *reinterpret_cast<uint2*>(dst + r * 256) = v;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (c0 + e < k) f[e] = Num<T>::to_f(src[e]);
+          if (c0 + r * 256 + e < q_cols) dst[r * 256 + e] = (uint8_t)((e < 4 ? v.x : v.y) >> (8 * (e & 3)));
       }
-    }
-    uint2 v;
-    const float s = fp8_block(f, v);
-    if (!live) continue;
-    if (lane16 == 0) scale[i] = s;
-    uint8_t* dst = q + row * q_stride + c0;
-    if (VEC && c0 + 8 <= q_cols) {
-      *reinterpret_cast<uint2*>(dst) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c0 + e < q_cols) dst[e] = (uint8_t)((e < 4 ? v.x : v.y) >> (8 * (e & 3)));
     }
   }
 }
@@ -59,18 +69,17 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
 template <typename T>
 static cudaError_t quantize_t(const void* x, int64_t x_stride, int64_t m, int64_t k, void* q, int64_t q_stride,
                               int64_t q_cols, float* scale, cudaStream_t st) {
-  const int kb = (int)((k + 127) / 128);
-  const int64_t nblk = m * kb;
-  int64_t grid = (nblk + 15) / 16;
-  if (grid > 148 * 8) grid = 148 * 8;
+  const int kb = (int)((k + 127) / 128), segs = (kb + 7) / 8;
+  int64_t grid = (m * segs + kQuantWarps - 1) / kQuantWarps;
+  if (grid > 148 * 32) grid = 148 * 32;
   const bool vec = ((uintptr_t)x % 16) == 0 && (x_stride * (int64_t)sizeof(T)) % 16 == 0 && ((uintptr_t)q % 8) == 0 &&
                    q_stride % 8 == 0;
   if (vec)
-    fp8_quantize_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>((const T*)x, x_stride, m, k, kb, (uint8_t*)q, q_stride,
-                                                                 q_cols, scale);
+    fp8_quantize_kernel<T, true><<<(unsigned)grid, kQuantWarps * 32, 0, st>>>(
+        (const T*)x, x_stride, m, k, kb, segs, (uint8_t*)q, q_stride, q_cols, scale);
   else
-    fp8_quantize_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>((const T*)x, x_stride, m, k, kb, (uint8_t*)q,
-                                                                  q_stride, q_cols, scale);
+    fp8_quantize_kernel<T, false><<<(unsigned)grid, kQuantWarps * 32, 0, st>>>(
+        (const T*)x, x_stride, m, k, kb, segs, (uint8_t*)q, q_stride, q_cols, scale);
   return cudaGetLastError();
 }
 

@@ -1,6 +1,7 @@
 // Shared by the 8-bit block-scaled kernels: the call's arguments, and the quantisation of one value block.
 #pragma once
 
+#include "fp32x2.cuh"
 #include "hga_common.cuh"
 
 namespace hga {
@@ -27,8 +28,7 @@ struct Fp8Linear {
 // which is larger than every finite value, so a NaN is never lost
 __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) {
-  const float amax = __uint_as_float(amax_bits);
+__device__ __forceinline__ float fp8_scale(float amax) {
   return amax <= 1e-30f ? 1.0f : __fdiv_rn(amax, 448.0f);  // NaN compares false: the scale is NaN
 }
 
@@ -38,34 +38,110 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   return r;
 }
 
-// 8 consecutive elements as fp32; p 16-byte aligned
+// 8 consecutive channels of a row as they are in memory.
+template <typename T> struct Raw8 {
+  uint4 u;
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+};
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+__device__ __forceinline__ Raw8<T> raw_zero() {
+  Raw8<T> r;
+  if constexpr (sizeof(T) == 4) r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
+  else r.u = make_uint4(0u, 0u, 0u, 0u);
+  return r;
+}
+// vec: p is 16-byte aligned; n of the 8 channels exist
+template <typename T>
+__device__ __forceinline__ Raw8<T> raw_load(const T* p, bool vec, int64_t n) {
+  Raw8<T> r = raw_zero<T>();
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      r.a = reinterpret_cast<const float4*>(p)[0];
+      r.b = reinterpret_cast<const float4*>(p)[1];
+    } else {
+      r.u = *reinterpret_cast<const uint4*>(p);
+    }
   } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&u);
+    T t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = e < n ? p[e] : Num<T>::from_f(0.f);
+    if constexpr (sizeof(T) == 4) {
+      r.a = make_float4(t[0], t[1], t[2], t[3]);
+      r.b = make_float4(t[4], t[5], t[6], t[7]);
+    } else {
+      r.u = *reinterpret_cast<const uint4*>(t);
+    }
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void raw_floats(const Raw8<T>& r, float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w;
+    f[4] = r.b.x; f[5] = r.b.y; f[6] = r.b.z; f[7] = r.b.w;
+  } else {
+    const T* h = reinterpret_cast<const T*>(&r.u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = Num<T>::to_f(h[i]);
   }
 }
+// Largest magnitude of the 16 lanes' channels as an integer (fp32 bits, or 16-bit bits), see mag_bits.
+template <typename T>
+__device__ __forceinline__ float raw_amax(const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t a = max(max(max(mag_bits(r.a.x), mag_bits(r.a.y)), max(mag_bits(r.a.z), mag_bits(r.a.w))),
+                     max(max(mag_bits(r.b.x), mag_bits(r.b.y)), max(mag_bits(r.b.z), mag_bits(r.b.w))));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    return __uint_as_float(a);
+  } else {
+    uint32_t a = __vmaxu2(__vmaxu2(r.u.x & 0x7fff7fffu, r.u.y & 0x7fff7fffu),
+                          __vmaxu2(r.u.z & 0x7fff7fffu, r.u.w & 0x7fff7fffu));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) a = __vmaxu2(a, __shfl_xor_sync(0xffffffffu, a, o));
+    const uint16_t h = (uint16_t)max(a & 0xffffu, a >> 16);
+    return Num<T>::to_f(*reinterpret_cast<const T*>(&h));
+  }
+}
+
+// e4m3 of the quotients f / s.  A quotient from the correctly rounded reciprocal by one exact remainder
+// (Markstein 1990: y = f r, q = y + (f - y s) r), three paired operations for two channels, where a plain
+// division takes about ten each.  It may differ from the IEEE quotient only where that lies within 2^-46
+// (relative) of the middle between two neighbouring floats; a quotient that is exactly on a boundary of
+// e4m3 comes out exactly.
+__device__ __forceinline__ uint2 fp8_quotients(const float (&f)[8], float s, float inv) {
+  uint16_t h[4];
+  const uint64_t r2 = f32x2(inv, inv), ns2 = f32x2(-s, -s);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint64_t f2 = f32x2(f[2 * e], f[2 * e + 1]);
+    const uint64_t y = f32x2_mul(f2, r2);
+    float lo, hi;
+    f32x2_get(f32x2_fma(f32x2_fma(y, ns2, f2), r2, y), lo, hi);
+    h[e] = e4m3x2(lo, hi);
+  }
+  return make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+}
+// The same by divisions: for a scale that is not finite, where the remainder is no number.
+static __device__ __noinline__ uint2 fp8_divisions(float a, float b, float c, float d, float e, float f, float g, float h,
+                                                   float s) {
+  return make_uint2(e4m3x2(__fdiv_rn(a, s), __fdiv_rn(b, s)) | (uint32_t)e4m3x2(__fdiv_rn(c, s), __fdiv_rn(d, s)) << 16,
+                    e4m3x2(__fdiv_rn(e, s), __fdiv_rn(f, s)) | (uint32_t)e4m3x2(__fdiv_rn(g, s), __fdiv_rn(h, s)) << 16);
+}
+__device__ __forceinline__ uint2 fp8_divisions(const float (&f)[8], float s) {
+  return fp8_divisions(f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7], s);
+}
 
 // The scale of a block of 128 channels held 8 a lane by 16 neighbouring lanes (all 32 lanes call), and the
 // lane's 8 e4m3 values.
-__device__ __forceinline__ float fp8_block(const float (&f)[8], uint2& v) {
-  uint32_t a = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) a = max(a, mag_bits(f[e]));
-#pragma unroll
-  for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-  const float s = fp8_scale(a);
-  uint16_t h[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = e4m3x2(__fdiv_rn(f[2 * e], s), __fdiv_rn(f[2 * e + 1], s));
-  v = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+template <typename T>
+__device__ __forceinline__ float fp8_block(const Raw8<T>& r, uint2& v) {
+  const float s = fp8_scale(raw_amax<T>(r));
+  float f[8];
+  raw_floats<T>(r, f);
+  v = s < INFINITY ? fp8_quotients(f, s, __frcp_rn(s)) : fp8_divisions(f, s);
   return s;
 }
 

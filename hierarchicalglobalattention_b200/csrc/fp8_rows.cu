@@ -141,37 +141,40 @@ __global__ void __launch_bounds__(kRowsThreads)
   } else {
     const int e = tid - 64;  // 0..127
     if constexpr (FUSED) {
-      // 16 lanes a block of 128 channels, 8 rows at a time; the operand's 128-byte swizzle: 16-byte piece p
-      // of row r sits at p ^ (r & 7)
+      // 16 lanes a block of 128 channels; the (block, row) pairs of the CTA's slice are dealt to the 8 half
+      // warps, four loads in flight each.  The operand's 128-byte swizzle: 16-byte piece p of row r sits at
+      // p ^ (r & 7).  Rows past m are zeros with scale 0.
       const TX* x = static_cast<const TX*>(a.x);
-      const int sub = e & 15, row8 = e >> 4;
-      constexpr int RPT = TN / 8;
-      for (int i = 0; i < nkb; ++i) {
-        const int c0 = (kb0 + i) * 128 + sub * 8;
-        float f[RPT][8];
+      const int sub = e & 15, live = a.m - t0 < TN ? a.m - t0 : TN, pairs = nkb * live;
+      constexpr int R = 4;
+      for (int i = e; i < nkb * (TN - live) * 8; i += 128) {
+        const int blk = i / ((TN - live) * 8), pc = i % ((TN - live) * 8);
+        *reinterpret_cast<uint4*>(smem + S::kXs + blk * S::kX + live * 128 + pc * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      for (int i = e; i < nkb * TN; i += 128) {
+        if (i % TN >= live) scale_s[i] = 0.f;
+      }
+      for (int base = (e >> 5) * 2; base < pairs; base += 8 * R) {
+        Raw8<TX> f[R];
 #pragma unroll
-        for (int j = 0; j < RPT; ++j) {
-          const int r = row8 + 8 * j;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) f[j][c] = 0.f;
-          if (t0 + r < a.m) {
-            const TX* src = x + (int64_t)(t0 + r) * a.x_stride + c0;
-            if (a.x_vec && c0 + 8 <= a.k) {
-              load8<TX>(src, f[j]);
-            } else {
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                if (c0 + c < a.k) f[j][c] = Num<TX>::to_f(src[c]);
-            }
-          }
+        for (int r = 0; r < R; ++r) {
+          const int pr = base + r * 8 + ((e >> 4) & 1);
+          const int c0 = (kb0 + pr / live) * 128 + sub * 8;
+          f[r] = pr < pairs ? raw_load<TX>(x + (int64_t)(t0 + pr % live) * a.x_stride + c0, a.x_vec, a.k - c0)
+                            : raw_zero<TX>();
         }
 #pragma unroll
-        for (int j = 0; j < RPT; ++j) {
-          const int r = row8 + 8 * j;
+        for (int r = 0; r < R; ++r) {
+          if (base + r * 8 >= pairs) break;  // warp-uniform
+          const int pr = base + r * 8 + ((e >> 4) & 1);
           uint2 v;
-          const float s = fp8_block(f[j], v);
-          *reinterpret_cast<uint2*>(smem + S::kXs + i * S::kX + r * 128 + (((sub >> 1) ^ (r & 7)) << 4) + (sub & 1) * 8) = v;
-          if (sub == 0) scale_s[i * TN + r] = s;
+          const float s = fp8_block<TX>(f[r], v);
+          if (pr < pairs) {
+            const int blk = pr / live, row = pr % live;
+            *reinterpret_cast<uint2*>(smem + S::kXs + blk * S::kX + row * 128 + (((sub >> 1) ^ (row & 7)) << 4) +
+                                      (sub & 1) * 8) = v;
+            if (sub == 0) scale_s[blk * TN + row] = s;
+          }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

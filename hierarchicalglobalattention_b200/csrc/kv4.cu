@@ -1,177 +1,342 @@
 // 4-bit KV record: pack, unpack, and the portable attention over it (any type, head_dim a multiple of 64).
 // The record's format is in kv4_common.cuh.
+#include <type_traits>
+
+#include "fp32x2.cuh"
 #include "kv4_common.cuh"
 
 namespace hga {
 
 HGA_DEVICE_ERROR_WORD(g_kv4_error, kv4_error_status)
 
+// ---- pack and unpack ------------------------------------------------------------------------------
+// 16 channels of one token as they are in memory, their extremes, and their values as pairs of fp32.
+template <typename T> struct Row16 {
+  uint4 u[2];
+};
+template <> struct Row16<float> {
+  uint4 u[4];
+};
 template <typename T>
-__device__ __forceinline__ void kv4_load8(const T* p, float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&u);
+__device__ __forceinline__ Row16<T> row16_load(const T* p, bool live) {
+  Row16<T> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Num<T>::to_f(h[i]);
+  for (int i = 0; i < (int)sizeof(T); ++i) r.u[i] = live ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0u, 0u, 0u, 0u);
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// a NaN among the channels makes both extremes NaN
+template <typename T>
+__device__ __forceinline__ void row16_extremes(const Row16<T>& r, float& lo, float& hi) {
+  if constexpr (sizeof(T) == 4) {
+    const float* f = reinterpret_cast<const float*>(r.u);
+    lo = hi = f[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      lo = min_nan(lo, f[i]);
+      hi = max_nan(hi, f[i]);
+    }
+  } else {
+    using V2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const V2* v = reinterpret_cast<const V2*>(r.u);
+    V2 l = v[0], h = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      l = __hmin2_nan(l, v[i]);
+      h = __hmax2_nan(h, v[i]);
+    }
+    lo = min_nan(Num<T>::to_f(l.x), Num<T>::to_f(l.y));
+    hi = max_nan(Num<T>::to_f(h.x), Num<T>::to_f(h.y));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void row16_pair(const Row16<T>& r, int i, float& a, float& b) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(r.u);
+  if constexpr (sizeof(T) == 4) {
+    a = __uint_as_float(w[2 * i]);
+    b = __uint_as_float(w[2 * i + 1]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(w + i));
+    a = f.x;
+    b = f.y;
+  } else {
+    a = __uint_as_float(w[i] << 16);
+    b = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
 
-constexpr int kPackWarps = 4;
+// What quantising one token's block needs: minimum, scale and its reciprocal; the (scale, min) word.
+struct Kv4Block {
+  float m, s, inv;
+  uint32_t word;
+};
+template <typename T>
+__device__ __forceinline__ Kv4Block kv4_block(float lo, float hi) {
+  using MT = typename Kv4Meta<T>::type;
+  const float odd = (lo - lo) + (hi - hi);  // 0, or NaN for a block with an infinity or a NaN
+  const MT pair[2] = {Num<MT>::from_f(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f) + odd), Num<MT>::from_f(lo + odd)};
+  Kv4Block b;
+  b.s = Num<MT>::to_f(pair[0]);
+  b.m = Num<MT>::to_f(pair[1]);
+  b.inv = __frcp_rn(b.s);
+  b.word = *reinterpret_cast<const uint32_t*>(pair);
+  return b;
+}
+// The codes of 16 channels, two to a word: codes[i] = n(2i) | n(2i + 1) << 16.  The quotient (x - m) / s comes
+// from the reciprocal and one exact remainder (Markstein 1990); adding 1.5 * 2^23 rounds it to an integer,
+// ties to even, in the low bits of the float.
+template <typename T>
+__device__ __forceinline__ void kv4_codes(const Row16<T>& r, const Kv4Block& b, uint32_t (&codes)[8]) {
+  // a scale that is normal in its type is within 2^-9 of the exact one and the minimum of a 16-bit cache is
+  // exact, so its quotients round to 0..15 by themselves
+  const bool plain = sizeof(T) == 2 && b.s >= (std::is_same<T, __half>::value ? 6.104e-5f : 1e-30f) && b.s < INFINITY;
+  const uint64_t nm = f32x2(-b.m, -b.m), inv = f32x2(b.inv, b.inv), ns = f32x2(-b.s, -b.s);
+  const uint64_t big = f32x2(12582912.f, 12582912.f), one = f32x2(1.f, 1.f);
+  if (plain) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x0, x1;
+      row16_pair<T>(r, i, x0, x1);
+      const uint64_t d = f32x2_fma(f32x2(x0, x1), one, nm);
+      const uint64_t y = f32x2_mul(d, inv);
+      const uint64_t q = f32x2_fma(f32x2_fma(f32x2_fma(y, ns, d), inv, y), one, big);
+      float q0, q1;
+      f32x2_get(q, q0, q1);
+      codes[i] = __byte_perm(__float_as_uint(q0), __float_as_uint(q1), 0x5410);
+    }
+  } else {
+    const bool usable = b.s > 0.f && b.s < INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x0, x1;
+      row16_pair<T>(r, i, x0, x1);
+      const float n0 = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x0, b.m), b.s)), 0.f), 15.f);
+      const float n1 = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x1, b.m), b.s)), 0.f), 15.f);
+      codes[i] = usable ? (uint32_t)(int)n0 | (uint32_t)(int)n1 << 16 : 0u;
+    }
+  }
+}
+// 4 x 4 transposition between 4 neighbouring lanes: w[k] of lane j becomes w[j] of lane k.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4], int j) {
+#pragma unroll
+  for (int s = 1; s < 4; s <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & s) continue;
+      const bool up = j & s;
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[i] : w[i + s], s);
+      if (up) w[i] = got; else w[i + s] = got;
+    }
+}
 
-// One warp per unit of K or of V.  The rows are read in their natural order (16-byte loads, 8 channels a
-// lane, a block of 32 channels in 4 neighbouring lanes), quantised, and their codes put as bytes in
-// shared memory, from which each lane assembles its words.  Bound by HBM.
+constexpr int kPackWarps = 8;
+
+// K: a warp takes a unit, four 16 x 16 tiles (64 channels) at a time; lane 4 g + j reads tokens g and g + 8
+// of tile j (two times 32 bytes), which is all that the words of lanes 4 g .. 4 g + 3 of that tile hold, and a
+// 4 x 4 transposition between neighbours brings each lane the four words that it stores as 16 bytes.
+// V: a half warp takes 64 channels of a unit; lane 4 c + j reads tokens 2c, 2c + 1, 2c + 8, 2c + 9 of tile j.
+// A block of 32 channels is two neighbouring lanes.  Bound by HBM; codes never pass through shared memory
+// (byte stores and nibble gathers there took three times as long).
 template <typename T, int DH>
 __global__ void __launch_bounds__(kPackWarps * 32) kv4_pack_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                                    int64_t bk, int64_t rows, int64_t cap,
                                                                    uint8_t* __restrict__ rec_k, uint8_t* __restrict__ rec_v,
                                                                    int64_t unit_cap, int64_t unit0) {
-  using MT = typename Kv4Meta<T>::type;
-  constexpr int LD = DH + 8;                 // bytes per staged code row
-  constexpr int LPR = DH / 8;                // lanes per row
-  __shared__ __align__(8) uint8_t stage[kPackWarps][16 * LD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t units = (rows + 15) / 16;
-  const int64_t total = 2 * bk * units;
-  uint8_t* sc = stage[warp];
-  for (int64_t w = (int64_t)blockIdx.x * kPackWarps + warp; w < total; w += (int64_t)gridDim.x * kPackWarps) {
-    const bool is_v = w >= bk * units;
-    const int64_t x = is_v ? w - bk * units : w;
-    const int64_t head = x / units, u = x - head * units;
-    const T* src = (is_v ? v : k) + (head * cap + u * 16) * DH;
-    uint8_t* dst = (is_v ? rec_v : rec_k) + (head * unit_cap + unit0 + u) * kv4_unit_bytes(DH);
-    uint32_t* meta = reinterpret_cast<uint32_t*>(dst + 8 * DH);
-    const int valid = rows - u * 16 < 16 ? (int)(rows - u * 16) : 16;
+  constexpr int QUADS = DH / 64, NB = DH / 32;
+  const int lane = threadIdx.x & 31, j = lane & 3;
+  const int64_t units = (rows + 15) / 16, n_k = bk * units, items_v = bk * units * QUADS, n_v = (items_v + 1) / 2;
+  for (int64_t w = (int64_t)blockIdx.x * kPackWarps + (threadIdx.x >> 5); w < n_k + n_v; w += (int64_t)gridDim.x * kPackWarps) {
+    if (w < n_k) {
+      const int64_t head = w / units, u = w - head * units;
+      const T* src = k + (head * cap + u * 16) * DH + j * 16;
+      uint8_t* dst = rec_k + (head * unit_cap + unit0 + u) * kv4_unit_bytes(DH);
+      uint32_t* meta = reinterpret_cast<uint32_t*>(dst + 8 * DH);
+      const int64_t left = rows - u * 16;
+      const int g = lane >> 2;
+      Row16<T> x[QUADS][2];
 #pragma unroll
-    for (int i = lane; i < 16 * LPR; i += 32) {
-      const int r = i / LPR, c8 = i % LPR;
-      float f[8];
-      if (r < valid) {
-        kv4_load8<T>(src + (int64_t)r * DH + c8 * 8, f);
-      } else {
+      for (int quad = 0; quad < QUADS; ++quad)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = 0.f;
-      }
-      float lo = f[0], hi = f[0], odd = 0.f;  // odd: NaN as soon as one value is not finite
+        for (int r = 0; r < 2; ++r) x[quad][r] = row16_load<T>(src + (int64_t)(g + 8 * r) * DH + quad * 64, g + 8 * r < left);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        lo = fminf(lo, f[e]);
-        hi = fmaxf(hi, f[e]);
-        odd += f[e] * 0.f;
-      }
+      for (int quad = 0; quad < QUADS; ++quad) {
+        uint32_t word[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        odd += __shfl_xor_sync(0xffffffffu, odd, o);
-      }
-      const MT mt = Num<MT>::from_f(lo + odd), st = Num<MT>::from_f(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f) + odd);
-      const float m = Num<MT>::to_f(mt), s = Num<MT>::to_f(st);
-      uint32_t codes[2] = {0u, 0u};
-      if (s > 0.f && s < INFINITY) {
+        for (int r = 0; r < 2; ++r) {
+          float lo, hi;
+          row16_extremes<T>(x[quad][r], lo, hi);
+          lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
+          hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+          const Kv4Block b = kv4_block<T>(lo, hi);
+          if ((j & 1) == r) meta[(g + 8 * r) * NB + quad * 2 + (j >> 1)] = b.word;
+          uint32_t n[8];
+          kv4_codes<T>(x[quad][r], b, n);
+          // channels 2c, 2c + 1 (pair c) and 8 + 2c, 9 + 2c (pair 4 + c): nibbles r, r + 4 and r + 2, r + 6
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float n = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(f[e], m), s)), 0.f), 15.f);
-          codes[e >> 2] |= (uint32_t)(int)n << (8 * (e & 3));
+          for (int c = 0; c < 4; ++c) word[c] += ((n[c] & 0x000f000fu) << (4 * r)) + ((n[4 + c] & 0x000f000fu) << (4 * r + 8));
         }
+        transpose4(word, j);
+        *reinterpret_cast<uint4*>(dst + (quad * 32 + lane) * 16) = make_uint4(word[0], word[1], word[2], word[3]);
       }
-      *reinterpret_cast<uint2*>(sc + r * LD + c8 * 8) = make_uint2(codes[0], codes[1]);
-      if ((c8 & 3) == 0) {
-        const MT pair[2] = {st, mt};
-        meta[r * (DH / 32) + c8 / 4] = *reinterpret_cast<const uint32_t*>(pair);
+    } else {
+      const int64_t item = (w - n_k) * 2 + (lane >> 4);
+      const bool on = item < items_v;
+      const int64_t it = on ? item : 0, unit = it / QUADS;
+      const int quad = (int)(it - unit * QUADS), c = (lane >> 2) & 3;
+      const int64_t head = unit / units, u = unit - head * units;
+      const T* src = v + (head * cap + u * 16) * DH + quad * 64 + j * 16;
+      uint8_t* dst = rec_v + (head * unit_cap + unit0 + u) * kv4_unit_bytes(DH);
+      uint32_t* meta = reinterpret_cast<uint32_t*>(dst + 8 * DH);
+      const int64_t left = rows - u * 16;
+      Row16<T> x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
+        x[i] = row16_load<T>(src + (int64_t)tok * DH, on && tok < left);
+      }
+      uint32_t word[8];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) word[g] = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
+        float lo, hi;
+        row16_extremes<T>(x[i], lo, hi);
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+        const Kv4Block b = kv4_block<T>(lo, hi);
+        if (on && (j & 1) == (i & 1)) meta[tok * NB + quad * 2 + (j >> 1)] = b.word;
+        uint32_t n[8];
+        kv4_codes<T>(x[i], b, n);
+        // token: nibble 4 * (tok % 2) + 2 * (tok / 8); channel g and g + 8 (pairs g / 2 and 4 + g / 2): + 0, + 1
+        constexpr uint32_t kLow = 0xfu;
+        const int sh = 16 * (i & 1) + 8 * (i >> 1);
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+          word[g] += ((n[g >> 1] >> (16 * (g & 1)) & kLow) << sh) + ((n[4 + (g >> 1)] >> (16 * (g & 1)) & kLow) << (sh + 4));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t t[4] = {word[4 * h], word[4 * h + 1], word[4 * h + 2], word[4 * h + 3]};
+        transpose4(t, j);  // channel row g = 4 h + j, tiles 0..3
+        if (on) *reinterpret_cast<uint4*>(dst + (quad * 32 + 4 * (4 * h + j) + c) * 16) = make_uint4(t[0], t[1], t[2], t[3]);
       }
     }
-    __syncwarp();
-    const int g = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int quad = 0; quad < DH / 64; ++quad) {
-      uint32_t word[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = quad * 4 + j;
-        uint32_t a = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int row = g + 8 * (e & 1), col = 2 * c + 8 * ((e >> 1) & 1) + (e >> 2);
-          const uint32_t n = is_v ? sc[col * LD + t * 16 + row] : sc[row * LD + t * 16 + col];
-          a |= n << (4 * e);
-        }
-        word[j] = a;
-      }
-      *reinterpret_cast<uint4*>(dst + (quad * 32 + lane) * 16) = make_uint4(word[0], word[1], word[2], word[3]);
-    }
-    __syncwarp();
   }
 }
 
-// The values of rows [0, rows): the mirror of kv4_pack_kernel.
+// 16 channels of a token from their codes as fp32 (scale * code + min: the product is exact).
+template <typename T>
+__device__ __forceinline__ void row16_store(T* p, const float (&n)[16], uint32_t word) {
+  using MT = typename Kv4Meta<T>::type;
+  const MT* pair = reinterpret_cast<const MT*>(&word);
+  const float s = Num<MT>::to_f(pair[0]), m = Num<MT>::to_f(pair[1]);
+  const uint64_t s2 = f32x2(s, s), m2 = f32x2(m, m);
+  T y[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float a, b;
+    f32x2_get(f32x2_fma(f32x2(n[2 * i], n[2 * i + 1]), s2, m2), a, b);
+    y[2 * i] = Num<T>::from_f(a);
+    y[2 * i + 1] = Num<T>::from_f(b);
+  }
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(y)[i];
+}
+__device__ __forceinline__ float nibble(uint32_t w, int i) {
+  return __uint_as_float((w >> (4 * i) & 15u) | 0x4b000000u) - 8388608.f;
+}
+
+// The values of rows [0, rows): kv4_pack_kernel backwards.
 template <typename T, int DH>
 __global__ void __launch_bounds__(kPackWarps * 32) kv4_unpack_kernel(const uint8_t* __restrict__ rec_k,
                                                                      const uint8_t* __restrict__ rec_v, int64_t unit_cap,
                                                                      int64_t unit0, int64_t bk, int64_t rows,
                                                                      T* __restrict__ k, T* __restrict__ v, int64_t cap) {
-  using MT = typename Kv4Meta<T>::type;
-  constexpr int LD = DH + 8;
-  constexpr int LPR = DH / 8;
-  __shared__ __align__(8) uint8_t stage[kPackWarps][16 * LD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t units = (rows + 15) / 16;
-  const int64_t total = 2 * bk * units;
-  uint8_t* sc = stage[warp];
-  for (int64_t w = (int64_t)blockIdx.x * kPackWarps + warp; w < total; w += (int64_t)gridDim.x * kPackWarps) {
-    const bool is_v = w >= bk * units;
-    const int64_t x = is_v ? w - bk * units : w;
-    const int64_t head = x / units, u = x - head * units;
-    const uint8_t* src = (is_v ? rec_v : rec_k) + (head * unit_cap + unit0 + u) * kv4_unit_bytes(DH);
-    T* dst = (is_v ? v : k) + (head * cap + u * 16) * DH;
-    const uint32_t* meta = reinterpret_cast<const uint32_t*>(src + 8 * DH);
-    const int valid = rows - u * 16 < 16 ? (int)(rows - u * 16) : 16;
-    const int g = lane >> 2, c = lane & 3;
+  constexpr int QUADS = DH / 64, NB = DH / 32;
+  const int lane = threadIdx.x & 31, j = lane & 3;
+  const int64_t units = (rows + 15) / 16, n_k = bk * units, items_v = bk * units * QUADS, n_v = (items_v + 1) / 2;
+  for (int64_t w = (int64_t)blockIdx.x * kPackWarps + (threadIdx.x >> 5); w < n_k + n_v; w += (int64_t)gridDim.x * kPackWarps) {
+    if (w < n_k) {
+      const int64_t head = w / units, u = w - head * units;
+      const uint8_t* src = rec_k + (head * unit_cap + unit0 + u) * kv4_unit_bytes(DH);
+      const uint32_t* meta = reinterpret_cast<const uint32_t*>(src + 8 * DH);
+      T* dst = k + (head * cap + u * 16) * DH + j * 16;
+      const int64_t left = rows - u * 16;
+      const int g = lane >> 2;
+      uint4 q4[QUADS];
+      uint32_t mw[QUADS][2];
 #pragma unroll
-    for (int quad = 0; quad < DH / 64; ++quad) {
-      const uint4 q4 = *reinterpret_cast<const uint4*>(src + (quad * 32 + lane) * 16);
-      const uint32_t word[4] = {q4.x, q4.y, q4.z, q4.w};
+      for (int quad = 0; quad < QUADS; ++quad) {
+        q4[quad] = *reinterpret_cast<const uint4*>(src + (quad * 32 + lane) * 16);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = quad * 4 + j;
+        for (int r = 0; r < 2; ++r) mw[quad][r] = meta[(g + 8 * r) * NB + quad * 2 + (j >> 1)];
+      }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int row = g + 8 * (e & 1), col = 2 * c + 8 * ((e >> 1) & 1) + (e >> 2);
-          sc[is_v ? col * LD + t * 16 + row : row * LD + t * 16 + col] = (uint8_t)((word[j] >> (4 * e)) & 15u);
+      for (int quad = 0; quad < QUADS; ++quad) {
+        uint32_t word[4] = {q4[quad].x, q4[quad].y, q4[quad].z, q4[quad].w};
+        transpose4(word, j);  // tile j: the words of lanes 4 g + c
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float n[16];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              n[2 * c + e] = nibble(word[c], r + 4 * e);
+              n[8 + 2 * c + e] = nibble(word[c], r + 2 + 4 * e);
+            }
+          if (g + 8 * r < left) row16_store<T>(dst + (int64_t)(g + 8 * r) * DH + quad * 64, n, mw[quad][r]);
         }
       }
-    }
-    __syncwarp();
+    } else {
+      const int64_t item = (w - n_k) * 2 + (lane >> 4);
+      const bool on = item < items_v;
+      const int64_t it = on ? item : 0, unit = it / QUADS;
+      const int quad = (int)(it - unit * QUADS), c = (lane >> 2) & 3;
+      const int64_t head = unit / units, u = unit - head * units;
+      const uint8_t* src = rec_v + (head * unit_cap + unit0 + u) * kv4_unit_bytes(DH);
+      const uint32_t* meta = reinterpret_cast<const uint32_t*>(src + 8 * DH);
+      T* dst = v + (head * cap + u * 16) * DH + quad * 64 + j * 16;
+      const int64_t left = rows - u * 16;
+      uint32_t word[8], mw[4];
 #pragma unroll
-    for (int i = lane; i < 16 * LPR; i += 32) {
-      const int r = i / LPR, c8 = i % LPR;
-      const uint2 n8 = *reinterpret_cast<const uint2*>(sc + r * LD + c8 * 8);
-      const uint32_t mw = meta[r * (DH / 32) + c8 / 4];
-      const MT* pair = reinterpret_cast<const MT*>(&mw);
-      const float s = Num<MT>::to_f(pair[0]), m = Num<MT>::to_f(pair[1]);
-      if (r < valid) {
-        T y[8];
+      for (int i = 0; i < 4; ++i) mw[i] = meta[(2 * c + (i & 1) + 8 * (i >> 1)) * NB + quad * 2 + (j >> 1)];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t n = ((e < 4 ? n8.x : n8.y) >> (8 * (e & 3))) & 255u;
-          y[e] = Num<T>::from_f(__fadd_rn(__fmul_rn((float)n, s), m));
+      for (int h = 0; h < 2; ++h) {
+        const uint4 q4 = *reinterpret_cast<const uint4*>(src + (quad * 32 + 4 * (4 * h + j) + c) * 16);
+        uint32_t t[4] = {q4.x, q4.y, q4.z, q4.w};
+        transpose4(t, j);  // tile j: channel rows 4 h + 0..3
+#pragma unroll
+        for (int e = 0; e < 4; ++e) word[4 * h + e] = t[e];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = 2 * c + (i & 1) + 8 * (i >> 1), nib = 4 * (i & 1) + 2 * (i >> 1);
+        float n[16];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          n[g] = nibble(word[g], nib);
+          n[8 + g] = nibble(word[g], nib + 1);
         }
-        uint4* o = reinterpret_cast<uint4*>(dst + (int64_t)r * DH + c8 * 8);
-        o[0] = reinterpret_cast<const uint4*>(y)[0];
-        if constexpr (sizeof(T) == 4) o[1] = reinterpret_cast<const uint4*>(y)[1];
+        if (on && tok < left) row16_store<T>(dst + (int64_t)tok * DH, n, mw[i]);
       }
     }
-    __syncwarp();
   }
 }
 
-static unsigned pack_grid(int64_t total) {
-  const int64_t ctas = (total + kPackWarps - 1) / kPackWarps;
-  return (unsigned)(ctas < 148 * 16 ? ctas : 148 * 16);
+static unsigned pack_grid(int64_t units, int dh) {
+  const int64_t ctas = (units + (units * (dh / 64) + 1) / 2 + kPackWarps - 1) / kPackWarps;
+  return (unsigned)(ctas < 148 * 64 ? ctas : 148 * 64);
 }
 
 #define HGA_KV4_DH(TT, CALL)                       \
@@ -192,7 +357,7 @@ static unsigned pack_grid(int64_t total) {
 
 cudaError_t launch_kv4_pack(int dtype, int dh, int64_t bk, int64_t rows, const void* k, const void* v, int64_t cap,
                             void* rec_k, void* rec_v, int64_t unit_cap, int64_t unit0, cudaStream_t st) {
-  const unsigned grid = pack_grid(2 * bk * ((rows + 15) / 16));
+  const unsigned grid = pack_grid(bk * ((rows + 15) / 16), dh);
   HGA_KV4_DISPATCH((kv4_pack_kernel<T, DH><<<grid, kPackWarps * 32, 0, st>>>(
       (const T*)k, (const T*)v, bk, rows, cap, (uint8_t*)rec_k, (uint8_t*)rec_v, unit_cap, unit0)))
   return cudaGetLastError();
@@ -200,7 +365,7 @@ cudaError_t launch_kv4_pack(int dtype, int dh, int64_t bk, int64_t rows, const v
 
 cudaError_t launch_kv4_unpack(int dtype, int dh, int64_t bk, int64_t rows, const void* rec_k, const void* rec_v,
                               int64_t unit_cap, int64_t unit0, void* k, void* v, int64_t cap, cudaStream_t st) {
-  const unsigned grid = pack_grid(2 * bk * ((rows + 15) / 16));
+  const unsigned grid = pack_grid(bk * ((rows + 15) / 16), dh);
   HGA_KV4_DISPATCH((kv4_unpack_kernel<T, DH><<<grid, kPackWarps * 32, 0, st>>>(
       (const uint8_t*)rec_k, (const uint8_t*)rec_v, unit_cap, unit0, bk, rows, (T*)k, (T*)v, cap)))
   return cudaGetLastError();
