@@ -288,7 +288,8 @@ static cudaError_t rows_t(const Fp8Linear& a, const void* q, int64_t q_stride, c
   r.bias = a.bias; r.out = a.out; r.out_stride = a.out_stride;
   const int smem = RowsSmem<TN, FUSED>::total((r.kb + r.splits - 1) / r.splits) + 1024;
   auto kern = fp8_rows_kernel<TX, TO, TN, FUSED>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static unsigned long long raised = 0;
+  cudaError_t e = raise_smem_limit((const void*)kern, RowsSmem<TN, FUSED>::total(kMaxSlice) + 1024, &raised);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(r.splits, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + TN - 1) / TN));

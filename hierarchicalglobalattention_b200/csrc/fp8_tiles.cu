@@ -294,7 +294,8 @@ static cudaError_t tiles_t(const Fp8Linear& a, const void* q, int64_t q_stride, 
   t.bias = a.bias; t.out = a.out; t.out_stride = a.out_stride; t.tma_out = tma_out;
   constexpr int smem = TileSmem<BN, STAGES>::kTotal + 1024;
   auto kern = fp8_tiles_kernel<T, BN, STAGES>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static unsigned long long raised = 0;
+  cudaError_t e = raise_smem_limit((const void*)kern, smem, &raised);
   if (e != cudaSuccess) return e;
   kern<<<t.tiles < 148 ? t.tiles : 148, kTileThreads, smem, st>>>(mx, mw, mo, t);
   return cudaGetLastError();

@@ -10,6 +10,19 @@
 
 namespace hga {
 
+// Raises a kernel's dynamic shared memory limit on the current device, once per device (`done`: one static
+// word per kernel, a bit per device): the attribute call costs as much host time as a launch.
+static inline cudaError_t raise_smem_limit(const void* kern, int bytes, unsigned long long* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(done, __ATOMIC_RELAXED) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) __atomic_fetch_or(done, bit, __ATOMIC_RELAXED);
+  return e;
+}
+
 // Finite mask fill of the reference (ExistingModelFineTuning/KvRouter/vectorized.py:38).
 constexpr float kNeg = -1.0e4f;
 

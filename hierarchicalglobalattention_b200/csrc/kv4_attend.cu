@@ -719,7 +719,8 @@ static cudaError_t launch_t(const hga_params& p, Args a, cudaStream_t st) {
   const int64_t z = (int64_t)a.heads_blk * a.tiles;
   if (z > 65535 || (int64_t)p.batch * p.kv_heads > 65535) return cudaErrorNotSupported;
   auto kern = attend_kv4_mma_kernel<T, DH, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static unsigned long long raised = 0;
+  cudaError_t e = raise_smem_limit((const void*)kern, 227 * 1024, &raised);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.splits, p.batch * p.kv_heads, (unsigned)z);

@@ -382,6 +382,10 @@ FP8_BLOCK = 128
 _FP8_X = {**_lib.DTYPE_CODE, torch.float8_e4m3fn: _lib.E4M3_CODE}
 
 
+# rows up to which hga_fp8_linear needs no workspace when its operands are 16-byte aligned
+_FP8_NO_WORKSPACE = 32
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x [..., K] as [M, K] rows with unit stride in the last dimension (a view where one exists)."""
     if x.dim() != 2:
@@ -392,18 +396,22 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [..., K] (fp32 / bf16 / fp16) as e4m3 values [..., K] and fp32 scales [..., ceil(K / 128)], one
     per row and block of 128 channels (see hga_fp8_quantize)."""
-    _require_cuda(x)
+    if not x.is_cuda:
+        _require_cuda(x)
     code = _lib.DTYPE_CODE.get(x.dtype)
-    if code is None or x.dim() == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if code is None or not shape or shape[-1] == 0:
         raise _lib.HgaError(f"fp8_quantize takes fp32 / bf16 / fp16 rows of at least one channel; got {x.dtype} "
-                            f"{tuple(x.shape)}")
-    K = x.shape[-1]
-    r = _rows(x)
-    M = r.shape[0]
-    q = torch.empty(*x.shape[:-1], K, device=x.device, dtype=torch.float8_e4m3fn)
-    scale = torch.empty(*x.shape[:-1], -(-K // FP8_BLOCK), device=x.device, dtype=torch.float32)
-    check(lib().hga_fp8_quantize(M, K, code, r.data_ptr(), max(r.stride(0), K), q.data_ptr(), K, scale.data_ptr(),
-                                 stream_ptr(x.device)), "hga_fp8_quantize")
+                            f"{tuple(shape)}")
+    K = shape[-1]
+    r = x if len(shape) == 2 and x.is_contiguous() else _rows(x)
+    dev = x.device
+    q = torch.empty(shape, device=dev, dtype=torch.float8_e4m3fn)
+    scale = torch.empty((*shape[:-1], -(-K // FP8_BLOCK)), device=dev, dtype=torch.float32)
+    rc = lib().hga_fp8_quantize(r.shape[0], K, code, r.data_ptr(), max(r.stride(0), K), q.data_ptr(), K,
+                                scale.data_ptr(), stream_ptr(dev))
+    if rc:
+        check(rc, "hga_fp8_quantize")
     return q, scale
 
 
@@ -432,21 +440,26 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     128 channels on the way in; e4m3 rows come with ``x_scale`` [..., ceil(K / 128)], as fp8_quantize
     returns them.  The result [..., N] has ``out_dtype``: x's type, or bf16 for 8-bit x.  ``bias`` [N] has
     the result's type."""
-    _require_cuda(x, w, w_scale, bias, x_scale)
+    dev = x.device
+    for t in (x, w, w_scale, bias, x_scale, out):
+        if t is not None and (not t.is_cuda or t.device != dev):
+            _require_cuda(t)
+            raise _lib.HgaError("fp8_linear: tensors on different devices")
     code = _FP8_X.get(x.dtype)
     if code is None:
         raise _lib.HgaError(f"fp8_linear: x must be fp32, bf16, fp16 or e4m3; got {x.dtype}")
     if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.stride(1) != 1:
         raise _lib.HgaError("fp8_linear: w must be an e4m3 [N, K] tensor with contiguous rows")
     N, K = w.shape
-    KB = -(-K // FP8_BLOCK)
-    if x.dim() == 0 or x.shape[-1] != K or K == 0 or N == 0:
-        raise _lib.HgaError(f"fp8_linear: x {tuple(x.shape)} does not fit w {tuple(w.shape)}")
-    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != (-(-N // FP8_BLOCK), KB) or w_scale.stride(1) != 1:
-        raise _lib.HgaError(f"fp8_linear: w_scale must be fp32 [{-(-N // FP8_BLOCK)}, {KB}] with contiguous rows")
+    KB, NB = -(-K // FP8_BLOCK), -(-N // FP8_BLOCK)
+    shape = x.shape
+    if not shape or shape[-1] != K or K == 0 or N == 0:
+        raise _lib.HgaError(f"fp8_linear: x {tuple(shape)} does not fit w {tuple(w.shape)}")
+    if w_scale.dtype != torch.float32 or w_scale.shape != (NB, KB) or w_scale.stride(1) != 1:
+        raise _lib.HgaError(f"fp8_linear: w_scale must be fp32 [{NB}, {KB}] with contiguous rows")
     xs = None
     if code == _lib.E4M3_CODE:
-        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (*x.shape[:-1], KB):
+        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != (*shape[:-1], KB):
             raise _lib.HgaError("fp8_linear: 8-bit x needs x_scale, fp32 [..., ceil(K / 128)]")
         xs = x_scale.contiguous()
         out_dtype = out_dtype or torch.bfloat16
@@ -458,22 +471,24 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
         raise _lib.HgaError(f"fp8_linear: out_dtype must be fp32, bf16 or fp16; got {out_dtype}")
     if bias is not None and (bias.dtype != out_dtype or bias.shape != (N,) or not bias.is_contiguous()):
         raise _lib.HgaError(f"fp8_linear: bias must be a contiguous [{N}] tensor of the result's type")
-    dev = x.device
-    for t in (w, w_scale, bias, xs, out):
-        if t is not None and t.device != dev:
-            raise _lib.HgaError("fp8_linear: tensors on different devices")
-    r = _rows(x)
+    r = x if len(shape) == 2 and x.is_contiguous() else _rows(x)
     M = r.shape[0]
     if out is None:
-        out = torch.empty(*x.shape[:-1], N, device=dev, dtype=out_dtype)
-    elif out.dtype != out_dtype or out.shape != (*x.shape[:-1], N) or not out.is_contiguous():
+        out = torch.empty((*shape[:-1], N), device=dev, dtype=out_dtype)
+    elif out.dtype != out_dtype or out.shape != (*shape[:-1], N) or not out.is_contiguous():
         raise _lib.HgaError("fp8_linear: out must be a contiguous [..., N] tensor of the result's type")
     h = lib()
     xp, wp, xst, wst = r.data_ptr(), w.data_ptr(), max(r.stride(0), K), max(w.stride(0), K)
-    need = h.hga_fp8_linear_workspace(M, N, K, code, xp, xst, wp, wst)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-    check(h.hga_fp8_linear(M, N, K, code, xp, xst, ptr(xs), wp, wst, w_scale.data_ptr(), max(w_scale.stride(0), KB),
-                           ptr(bias), ocode, out.data_ptr(), N, ptr(ws), need, stream_ptr(dev)), "hga_fp8_linear")
+    need, ws = 0, None
+    if M > _FP8_NO_WORKSPACE or code == _lib.E4M3_CODE or (wp | wst) & 15 or K > 16384:
+        need = h.hga_fp8_linear_workspace(M, N, K, code, xp, xst, wp, wst)
+        if need:
+            ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    rc = h.hga_fp8_linear(M, N, K, code, xp, xst, None if xs is None else xs.data_ptr(), wp, wst, w_scale.data_ptr(),
+                          max(w_scale.stride(0), KB), None if bias is None else bias.data_ptr(), ocode, out.data_ptr(),
+                          N, None if ws is None else ws.data_ptr(), need, stream_ptr(dev))
+    if rc:
+        check(rc, "hga_fp8_linear")
     return out
 
 
@@ -490,20 +505,23 @@ def kv4_unit_bytes(head_dim: int) -> int:
 
 def _kv4_rec(name: str, rec: torch.Tensor, B: int, KVH: int, Dh: int) -> int:
     """Units allocated per (sequence, KV head) of a record [B, KVH, units, 10 * Dh]."""
-    if (rec.dtype != torch.uint8 or rec.dim() != 4 or rec.shape[0] != B or rec.shape[1] != KVH
-            or rec.shape[3] != 10 * Dh or not rec.is_contiguous()):
+    shape = rec.shape
+    if (rec.dtype != torch.uint8 or len(shape) != 4 or shape[0] != B or shape[1] != KVH or shape[3] != 10 * Dh
+            or not rec.is_contiguous()):
         raise _lib.HgaError(f"{name}: a record is a contiguous uint8 [B, KVH, units, 10 * Dh] tensor; got {rec.dtype} "
-                            f"{tuple(rec.shape)} for B={B}, KVH={KVH}, Dh={Dh}")
-    if rec.device.type != "cuda" and not rec.is_pinned():
+                            f"{tuple(shape)} for B={B}, KVH={KVH}, Dh={Dh}")
+    if not rec.is_cuda and not rec.is_pinned():
         raise _lib.HgaError(f"{name}: a record in host memory must be pinned")
-    return rec.shape[2]
+    return shape[2]
 
 
 def _kv4_rows(t: torch.Tensor) -> torch.Tensor:
     """K/V rows as a row-slice of a contiguous [B,KVH,cap,Dh] buffer (copied when they are laid out otherwise)."""
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t
     B, KVH, S, Dh = t.shape
-    ok = (t.stride(3) == 1 and t.stride(2) == Dh and t.stride(1) % Dh == 0 and t.stride(1) >= S * Dh
-          and t.stride(0) == KVH * t.stride(1) and t.data_ptr() % 16 == 0)
+    s0, s1, s2, s3 = t.stride()
+    ok = s3 == 1 and s2 == Dh and s1 % Dh == 0 and s1 >= S * Dh and s0 == KVH * s1 and not t.data_ptr() & 15
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -530,8 +548,10 @@ def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor,
     k, v = _kv4_rows(k), _kv4_rows(v)
     if k.stride(1) != v.stride(1):
         k, v = k.contiguous(), v.contiguous()
-    check(lib().hga_kv4_pack(_lib.DTYPE_CODE[k.dtype], Dh, B * KVH, S, k.data_ptr(), v.data_ptr(), k.stride(1) // Dh,
-                             rec_k.data_ptr(), rec_v.data_ptr(), cap, unit0, stream_ptr(k.device)), "hga_kv4_pack")
+    rc = lib().hga_kv4_pack(_lib.DTYPE_CODE[k.dtype], Dh, B * KVH, S, k.data_ptr(), v.data_ptr(), k.stride(1) // Dh,
+                            rec_k.data_ptr(), rec_v.data_ptr(), cap, unit0, stream_ptr(k.device))
+    if rc:
+        check(rc, "hga_kv4_pack")
     return rec_k, rec_v
 
 
@@ -553,8 +573,10 @@ def kv4_unpack(rec_k: torch.Tensor, rec_v: torch.Tensor, seq_len: int, dtype: to
         raise _lib.HgaError("hga ops run on CUDA tensors only (no CPU fallback): give kv4_unpack a CUDA device")
     k = torch.empty(B, KVH, seq_len, Dh, device=dev, dtype=dtype)
     v = torch.empty_like(k)
-    check(lib().hga_kv4_unpack(_lib.DTYPE_CODE[dtype], Dh, B * KVH, seq_len, rec_k.data_ptr(), rec_v.data_ptr(), cap,
-                               unit0, k.data_ptr(), v.data_ptr(), seq_len, stream_ptr(dev)), "hga_kv4_unpack")
+    rc = lib().hga_kv4_unpack(_lib.DTYPE_CODE[dtype], Dh, B * KVH, seq_len, rec_k.data_ptr(), rec_v.data_ptr(), cap,
+                              unit0, k.data_ptr(), v.data_ptr(), seq_len, stream_ptr(dev))
+    if rc:
+        check(rc, "hga_kv4_unpack")
     return k, v
 
 
@@ -587,10 +609,12 @@ def attend_decode_kv4(p: HgaParams, q: torch.Tensor, seq_pos: torch.Tensor, hot_
     hot_cap = kv_cap_of(hot_k)
     if kv_cap_of(hot_v) != hot_cap:
         raise _lib.HgaError("attend_decode_kv4: hot_k and hot_v must share one capacity layout")
-    check(lib().hga_attend_decode_kv4(ctypes_params(p), L, q.data_ptr(), seq_pos.data_ptr(), hot_k.data_ptr(),
-                                      hot_v.data_ptr(), hot_cap, rec_k.data_ptr(), rec_v.data_ptr(), cap,
-                                      open_gid.data_ptr(), open_t0.data_ptr(), open_gid.shape[2], out.data_ptr(),
-                                      stream_ptr(q.device)), "hga_attend_decode_kv4")
+    rc = lib().hga_attend_decode_kv4(ctypes_params(p), L, q.data_ptr(), seq_pos.data_ptr(), hot_k.data_ptr(),
+                                     hot_v.data_ptr(), hot_cap, rec_k.data_ptr(), rec_v.data_ptr(), cap,
+                                     open_gid.data_ptr(), open_t0.data_ptr(), open_gid.shape[2], out.data_ptr(),
+                                     stream_ptr(q.device))
+    if rc:
+        check(rc, "hga_attend_decode_kv4")
     return out
 
 
