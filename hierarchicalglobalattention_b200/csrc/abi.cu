@@ -466,7 +466,7 @@ int hga_fp8_quantize(int64_t m, int64_t k, int32_t dtype, const void* x, int64_t
   if (m == 0) return HGA_OK;
   if (!x || !q || !scale) return fail(HGA_E_INVALID, "hga_fp8_quantize: NULL tensor");
   if (x_stride < k || q_stride < k) return fail(HGA_E_INVALID, "hga_fp8_quantize: row stride smaller than the row");
-  return cuda_status(hga::launch_fp8_quantize(dtype, x, x_stride, m, k, q, q_stride, k, scale, stream),
+  return cuda_status(hga::launch_fp8_quantize(dtype, x, x_stride, m, k, q, q_stride, k, scale, (k + 127) / 128, stream),
                      "hga_fp8_quantize");
 }
 

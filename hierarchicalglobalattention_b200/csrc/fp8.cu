@@ -23,7 +23,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quantize_kernel(const T* __restrict__ x, int64_t x_stride,
                                                                         int64_t m, int64_t k, int kb, int segs,
                                                                         uint8_t* __restrict__ q, int64_t q_stride,
-                                                                        int64_t q_cols, float* __restrict__ scale) {
+                                                                        int64_t q_cols, float* __restrict__ scale,
+                                                                        int64_t scale_stride) {
   const int lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
   const int64_t tasks = m * segs, step = (int64_t)gridDim.x * kQuantWarps;
   for (int64_t task = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5); task < tasks; task += step) {
@@ -43,7 +44,7 @@ __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quantize_kernel(const T*
     }
     const float my_s = fp8_scale(mine), my_inv = __frcp_rn(my_s);
     const bool odd = __any_sync(0xffffffffu, !(my_s < INFINITY));
-    if (sub < 4 && blk0 + 2 * sub < kb) scale[row * kb + blk0 + 2 * sub] = my_s;
+    if (sub < 4 && blk0 + 2 * sub < kb) scale[row * scale_stride + blk0 + 2 * sub] = my_s;
     uint8_t* dst = q + row * q_stride + c0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(kQuantWarps * 32) fp8_quantize_kernel(const T*
 
 template <typename T>
 static cudaError_t quantize_t(const void* x, int64_t x_stride, int64_t m, int64_t k, void* q, int64_t q_stride,
-                              int64_t q_cols, float* scale, cudaStream_t st) {
+                              int64_t q_cols, float* scale, int64_t scale_stride, cudaStream_t st) {
   const int kb = (int)((k + 127) / 128), segs = (kb + 7) / 8;
   int64_t grid = (m * segs + kQuantWarps - 1) / kQuantWarps;
   if (grid > 148 * 32) grid = 148 * 32;
@@ -76,20 +77,20 @@ static cudaError_t quantize_t(const void* x, int64_t x_stride, int64_t m, int64_
                    q_stride % 8 == 0;
   if (vec)
     fp8_quantize_kernel<T, true><<<(unsigned)grid, kQuantWarps * 32, 0, st>>>(
-        (const T*)x, x_stride, m, k, kb, segs, (uint8_t*)q, q_stride, q_cols, scale);
+        (const T*)x, x_stride, m, k, kb, segs, (uint8_t*)q, q_stride, q_cols, scale, scale_stride);
   else
     fp8_quantize_kernel<T, false><<<(unsigned)grid, kQuantWarps * 32, 0, st>>>(
-        (const T*)x, x_stride, m, k, kb, segs, (uint8_t*)q, q_stride, q_cols, scale);
+        (const T*)x, x_stride, m, k, kb, segs, (uint8_t*)q, q_stride, q_cols, scale, scale_stride);
   return cudaGetLastError();
 }
 
 // q_cols >= k columns are written: channels past k are zeros
 cudaError_t launch_fp8_quantize(int dtype, const void* x, int64_t x_stride, int64_t m, int64_t k, void* q,
-                                int64_t q_stride, int64_t q_cols, float* scale, cudaStream_t st) {
+                                int64_t q_stride, int64_t q_cols, float* scale, int64_t scale_stride, cudaStream_t st) {
   switch (dtype) {
-    case HGA_DTYPE_F32: return quantize_t<float>(x, x_stride, m, k, q, q_stride, q_cols, scale, st);
-    case HGA_DTYPE_BF16: return quantize_t<__nv_bfloat16>(x, x_stride, m, k, q, q_stride, q_cols, scale, st);
-    case HGA_DTYPE_F16: return quantize_t<__half>(x, x_stride, m, k, q, q_stride, q_cols, scale, st);
+    case HGA_DTYPE_F32: return quantize_t<float>(x, x_stride, m, k, q, q_stride, q_cols, scale, scale_stride, st);
+    case HGA_DTYPE_BF16: return quantize_t<__nv_bfloat16>(x, x_stride, m, k, q, q_stride, q_cols, scale, scale_stride, st);
+    case HGA_DTYPE_F16: return quantize_t<__half>(x, x_stride, m, k, q, q_stride, q_cols, scale, scale_stride, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -119,6 +120,9 @@ static cudaError_t realign(const void* src, int64_t stride, int64_t rows, int64_
 
 static bool off_grid(const void* p, int64_t stride) { return ((uintptr_t)p & 15) || (stride & 15); }
 
+// Floats between the scales of two rows in the workspace: whole 16-byte pieces.
+static int64_t scale_stride(int64_t kb) { return (kb + 3) / 4 * 4; }
+
 // Workspace: [quantised or realigned x][its scales][realigned w], each part present only where needed.
 static void parts(const Fp8Linear& a, int64_t& xq, int64_t& xs, int64_t& w) {
   const int64_t kb = (a.k + 127) / 128;
@@ -126,7 +130,7 @@ static void parts(const Fp8Linear& a, int64_t& xq, int64_t& xs, int64_t& w) {
   if (a.x_dtype != HGA_DTYPE_E4M3) {
     if (!fp8_rows_fused(a)) {
       xq = a.m * kb * 128;
-      xs = (a.m * kb * 4 + 15) / 16 * 16;
+      xs = a.m * scale_stride(kb) * 4;
     }
   } else if (off_grid(a.x, a.x_stride)) {
     xq = a.m * kb * 128;
@@ -148,6 +152,7 @@ cudaError_t launch_fp8_linear(const Fp8Linear& a, cudaStream_t st) {
   const void* q = a.x;
   int64_t q_stride = a.x_stride;
   const float* xs = a.x_scale;
+  int64_t xs_stride = cols / 128;
   const void* w = a.w;
   int64_t w_stride = a.w_stride;
   cudaError_t e = cudaSuccess;
@@ -156,7 +161,8 @@ cudaError_t launch_fp8_linear(const Fp8Linear& a, cudaStream_t st) {
     q_stride = cols;
     if (xsb) {
       xs = (const float*)(ws + xqb);
-      e = launch_fp8_quantize(a.x_dtype, a.x, a.x_stride, a.m, a.k, ws, cols, cols, (float*)(ws + xqb), st);
+      xs_stride = scale_stride(cols / 128);
+      e = launch_fp8_quantize(a.x_dtype, a.x, a.x_stride, a.m, a.k, ws, cols, cols, (float*)(ws + xqb), xs_stride, st);
     } else {
       e = realign(a.x, a.x_stride, a.m, a.k, ws, cols, st);
     }
@@ -168,8 +174,8 @@ cudaError_t launch_fp8_linear(const Fp8Linear& a, cudaStream_t st) {
     e = realign(a.w, a.w_stride, a.n, a.k, ws + xqb + xsb, cols, st);
     if (e != cudaSuccess) return e;
   }
-  if (fp8_rows_better(a)) return launch_fp8_rows(a, q, q_stride, xs, w, w_stride, st);
-  return launch_fp8_tiles(a, q, q_stride, xs, w, w_stride, st);
+  if (fp8_rows_better(a)) return launch_fp8_rows(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  return launch_fp8_tiles(a, q, q_stride, xs, xs_stride, w, w_stride, st);
 }
 
 }  // namespace hga

@@ -146,15 +146,15 @@ __device__ __forceinline__ float fp8_block(const Raw8<T>& r, uint2& v) {
 }
 
 cudaError_t launch_fp8_quantize(int dtype, const void* x, int64_t x_stride, int64_t m, int64_t k, void* q,
-                                int64_t q_stride, int64_t q_cols, float* scale, cudaStream_t st);
+                                int64_t q_stride, int64_t q_cols, float* scale, int64_t scale_stride, cudaStream_t st);
 
 // The products on the tensor cores.  q [m][k] e4m3 and w: 16-byte aligned bases and row strides.
-cudaError_t launch_fp8_tiles(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                             int64_t w_stride, cudaStream_t st);
+cudaError_t launch_fp8_tiles(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                             const void* w, int64_t w_stride, cudaStream_t st);
 // Few rows: quantises x itself (x_dtype not E4M3) or takes q / xs.
 bool fp8_rows_fused(const Fp8Linear& a);
 bool fp8_rows_better(const Fp8Linear& a);
-cudaError_t launch_fp8_rows(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                            int64_t w_stride, cudaStream_t st);
+cudaError_t launch_fp8_rows(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                            const void* w, int64_t w_stride, cudaStream_t st);
 
 }  // namespace hga

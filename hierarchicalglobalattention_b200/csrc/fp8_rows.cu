@@ -29,6 +29,7 @@ struct RowsArgs {
   int64_t x_stride;
   int x_vec;          // 16-byte loads are possible
   const float* xs;    // not FUSED: their scales
+  int64_t xs_stride;
   const float* ws;
   int64_t ws_stride;
   const void* bias;
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(kRowsThreads)
     } else {
       for (int i = e; i < nkb * TN; i += 128) {
         const int r = t0 + i % TN;
-        scale_s[i] = r < a.m ? a.xs[(int64_t)r * a.kb + kb0 + i / TN] : 0.f;
+        scale_s[i] = r < a.m ? a.xs[(int64_t)r * a.xs_stride + kb0 + i / TN] : 0.f;
       }
     }
     mbar_arrive(x_ready);
@@ -265,8 +266,8 @@ static int rows_splits(int64_t m, int64_t n, int64_t kb, int tn) {
 static int rows_tn(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
 
 template <typename TX, typename TO, int TN, bool FUSED>
-static cudaError_t rows_t(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                          int64_t w_stride, cudaStream_t st) {
+static cudaError_t rows_t(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                          const void* w, int64_t w_stride, cudaStream_t st) {
   CUtensorMap mx, mw;
   const cuuint64_t dw[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n}, sw[1] = {(cuuint64_t)w_stride};
   const cuuint32_t bw[2] = {128, 128};
@@ -284,7 +285,7 @@ static cudaError_t rows_t(const Fp8Linear& a, const void* q, int64_t q_stride, c
   r.splits = rows_splits(a.m, a.n, r.kb, TN);
   r.x = a.x; r.x_stride = a.x_stride;
   r.x_vec = ((uintptr_t)a.x & 15) == 0 && (a.x_stride * (int64_t)sizeof(TX)) % 16 == 0;
-  r.xs = xs; r.ws = a.w_scale; r.ws_stride = a.ws_stride;
+  r.xs = xs; r.xs_stride = xs_stride; r.ws = a.w_scale; r.ws_stride = a.ws_stride;
   r.bias = a.bias; r.out = a.out; r.out_stride = a.out_stride;
   const int smem = RowsSmem<TN, FUSED>::total((r.kb + r.splits - 1) / r.splits) + 1024;
   auto kern = fp8_rows_kernel<TX, TO, TN, FUSED>;
@@ -306,23 +307,23 @@ static cudaError_t rows_t(const Fp8Linear& a, const void* q, int64_t q_stride, c
 }
 
 template <typename TX, typename TO, bool FUSED>
-static cudaError_t rows_m(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                          int64_t w_stride, cudaStream_t st) {
+static cudaError_t rows_m(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                          const void* w, int64_t w_stride, cudaStream_t st) {
   const int tn = rows_tn(a.m);
-  if (tn == 16) return rows_t<TX, TO, 16, FUSED>(a, q, q_stride, xs, w, w_stride, st);
-  if (tn == 32) return rows_t<TX, TO, 32, FUSED>(a, q, q_stride, xs, w, w_stride, st);
-  if constexpr (!FUSED) return rows_t<TX, TO, 64, false>(a, q, q_stride, xs, w, w_stride, st);
+  if (tn == 16) return rows_t<TX, TO, 16, FUSED>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  if (tn == 32) return rows_t<TX, TO, 32, FUSED>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  if constexpr (!FUSED) return rows_t<TX, TO, 64, false>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
   return cudaErrorInvalidValue;
 }
 
 template <typename TO>
-static cudaError_t rows_o(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                          int64_t w_stride, cudaStream_t st) {
-  if (!fp8_rows_fused(a)) return rows_m<TO, TO, false>(a, q, q_stride, xs, w, w_stride, st);
+static cudaError_t rows_o(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                          const void* w, int64_t w_stride, cudaStream_t st) {
+  if (!fp8_rows_fused(a)) return rows_m<TO, TO, false>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
   switch (a.x_dtype) {
-    case HGA_DTYPE_F32: return rows_m<float, TO, true>(a, q, q_stride, xs, w, w_stride, st);
-    case HGA_DTYPE_BF16: return rows_m<__nv_bfloat16, TO, true>(a, q, q_stride, xs, w, w_stride, st);
-    case HGA_DTYPE_F16: return rows_m<__half, TO, true>(a, q, q_stride, xs, w, w_stride, st);
+    case HGA_DTYPE_F32: return rows_m<float, TO, true>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+    case HGA_DTYPE_BF16: return rows_m<__nv_bfloat16, TO, true>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+    case HGA_DTYPE_F16: return rows_m<__half, TO, true>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -339,12 +340,12 @@ bool fp8_rows_better(const Fp8Linear& a) { return a.m <= 256 && rows_fit(a); }
 
 bool fp8_rows_fused(const Fp8Linear& a) { return a.x_dtype != HGA_DTYPE_E4M3 && a.m <= 32 && rows_fit(a); }
 
-cudaError_t launch_fp8_rows(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                            int64_t w_stride, cudaStream_t st) {
+cudaError_t launch_fp8_rows(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                            const void* w, int64_t w_stride, cudaStream_t st) {
   switch (a.out_dtype) {
-    case HGA_DTYPE_F32: return tc::rows_o<float>(a, q, q_stride, xs, w, w_stride, st);
-    case HGA_DTYPE_BF16: return tc::rows_o<__nv_bfloat16>(a, q, q_stride, xs, w, w_stride, st);
-    case HGA_DTYPE_F16: return tc::rows_o<__half>(a, q, q_stride, xs, w, w_stride, st);
+    case HGA_DTYPE_F32: return tc::rows_o<float>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+    case HGA_DTYPE_BF16: return tc::rows_o<__nv_bfloat16>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+    case HGA_DTYPE_F16: return tc::rows_o<__half>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
   }
   return cudaErrorInvalidValue;
 }

@@ -5,11 +5,13 @@
 // The scales change every 128 channels, so a block's products cannot stay in the accumulator: each
 // block is one MMA group of four K = 32 steps into one of two TMEM buffers, and eight epilogue warps
 // add it, scaled, to fp32 sums in registers (one fp32 FMA per output and block) while the tensor cores
-// work on the next block in the other buffer.  Persistent CTAs, one per SM, walk the output tiles with
-// neighbouring feature tiles first (their rows of x are then read from L2).
-//   warp 0      TMA producer: 128 x 128 bytes of x and BN x 128 bytes of w per block, STAGES deep, SW128
-//   warp 1      MMA issuer (one lane), TMEM owner
-//   warps 2-9   each reads 32 TMEM lanes (rows) x BN / 2 columns: one row a thread, one weight block a
+// work on the next block in the other buffer.  Persistent CTAs walk the output tiles with neighbouring
+// feature tiles first (their rows of x are then read from L2).  Large products run as pairs of CTAs on
+// 256 x 256 tiles (cta_group::2): every CTA loads its own 128 rows and half of the features, 32 KB a block
+// where a single CTA's 128 x 256 tile needs 48.
+//   warp 0      TMA producer: x and w of one block per stage, STAGES deep, SW128
+//   warp 1      MMA issuer (of the even CTA), TMEM owner
+//   warps 4-11  each reads 32 TMEM lanes (rows) x BN / 2 columns: one row a thread, one weight block a
 //               warp, so a block's scale is one product per thread
 // Results go through 4 KB of swizzled shared memory per warp to whole-line TMA stores (plain stores where
 // the output's rows are off the 16-byte grid).  Waits are bounded as in tc_common.cuh.
@@ -19,12 +21,15 @@
 namespace hga {
 namespace tc {
 
-constexpr int kTileThreads = 320;
-constexpr int kErrFp8 = 0x40;  // codes 0x40..0x47 of the bounded waits
+constexpr int kEpiWarps = 8;
+constexpr int kTileThreads = 128 + 32 * kEpiWarps;
+constexpr int kErrFp8 = 0x40;      // codes 0x40..0x47 of the bounded waits
 
 struct TileArgs {
   int m, n, kb, tiles_n, tiles;
   const float* xs;
+  int64_t xs_stride;  // floats between rows
+  int xs_vec;         // rows are 16-byte aligned and padded to whole float4
   const float* ws;
   int64_t ws_stride;
   const void* bias;
@@ -33,28 +38,28 @@ struct TileArgs {
   int tma_out;
 };
 
-template <int BN, int STAGES> struct TileSmem {
-  static constexpr int kA = 128 * 128, kB = BN * 128;
+// The scales of 4 blocks from block kb on (0 past the end).
+__device__ __forceinline__ float4 scales4(const float* p, int kb, int n, bool vec) {
+  if (vec) return kb < n ? *reinterpret_cast<const float4*>(p + kb) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 v;
+  v.x = kb < n ? p[kb] : 0.f;
+  v.y = kb + 1 < n ? p[kb + 1] : 0.f;
+  v.z = kb + 2 < n ? p[kb + 2] : 0.f;
+  v.w = kb + 3 < n ? p[kb + 3] : 0.f;
+  return v;
+}
+
+// PAIR CTAs make one tile of 128 * PAIR rows x BN features; each loads its 128 rows of x and BN / PAIR
+// features of w per block.
+template <int BN, int PAIR, int STAGES> struct TileSmem {
+  static constexpr int kA = 128 * 128, kB = BN / PAIR * 128;
   static constexpr int kStage = kA + kB;
-  static constexpr int kOut = STAGES * kStage;       // 8 x 4 KB
-  static constexpr int kBars = kOut + 8 * 4096;
-  static constexpr int kMisc = kBars + (2 * STAGES + 5) * 8;
+  static constexpr int kOut = STAGES * kStage;       // 4 KB per epilogue warp
+  static constexpr int kBars = kOut + kEpiWarps * 4096;
+  static constexpr int kMisc = kBars + (2 * STAGES + 3) * 8;
   static constexpr int kTotal = kMisc + 32;
 };
 
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
                "r"(smem_u32(src))
@@ -63,6 +68,17 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// One lane of the warp, the same one every time; all lanes call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack_out(float a, float b) {
@@ -74,127 +90,176 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
   }
 }
 
-template <typename T, int BN, int STAGES>
+template <typename T, int BN, int PAIR, int STAGES>
 __global__ void __launch_bounds__(kTileThreads, 1)
     fp8_tiles_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                      const __grid_constant__ CUtensorMap tm_o, const TileArgs a) {
-  using S = TileSmem<BN, STAGES>;
+  using S = TileSmem<BN, PAIR, STAGES>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-  uint64_t* full = bars;
-  uint64_t* empty = bars + STAGES;
-  uint64_t* d_full = bars + 2 * STAGES;       // [2]
-  uint64_t* d_empty = bars + 2 * STAGES + 2;  // [2]
-  uint64_t* drain = bars + 2 * STAGES + 4;
+  uint64_t* full = bars;                      // the even CTA's counts the bytes of both
+  uint64_t* done = bars + STAGES;             // the MMAs of a stage: its operands are free and its block is in TMEM
+  uint64_t* d_empty = bars + 2 * STAGES;      // [2] the even CTA's counts the epilogue warps of both
+  uint64_t* drain = bars + 2 * STAGES + 2;
   int* misc = reinterpret_cast<int*>(smem + S::kMisc);
   volatile int* abort_flag = misc;
   uint32_t* tmem_s = reinterpret_cast<uint32_t*>(misc + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR == 2 ? blockIdx.x & 1 : 0, group = blockIdx.x / PAIR, groups = gridDim.x / PAIR;
 
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
+      mbar_init(done + i, 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(d_full + i, 1);
-      mbar_init(d_empty + i, 8);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(d_empty + i, kEpiWarps * PAIR);
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort_flag = 0;
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_s)),
-                 "r"(2u * BN));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (PAIR == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_s)),
+                   "r"(2u * BN));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_s)),
+                   "r"(2u * BN));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   fence_before();
   __syncthreads();
+  if constexpr (PAIR == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = *tmem_s;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
+  // registers: 384 threads x 168 at launch = 128 x 40 (the producers' group) + 256 x 232 (the epilogue: 128
+  // sums, a 64-column read, the scales ahead; a spilled register would come from L2).  In the branches
+  // themselves: after a join the compiler would hold every role to the smaller count.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // The producer and MMA warps run their loops as whole warps with one elected lane issuing: the loop
+    // state, addresses and descriptors are then uniform.  (From a single-lane branch every operand of an
+    // MMA was moved to a uniform register first, 90 cycles an instruction.)
+    const bool leader = elect_one();
+    if (warp == 0) {
+      int st = 0, it = 0;
+      uint32_t phase = 1;  // the first round finds the stages empty
       bool ok = true;
-      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
-        const int m0 = tile / a.tiles_n * 128, n0 = tile % a.tiles_n * BN;
+      for (int tile = group; tile < a.tiles && ok; tile += groups) {
+        const int m0 = tile / a.tiles_n * (128 * PAIR) + rank * 128, n0 = tile % a.tiles_n * BN + rank * (BN / PAIR);
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
-          const int st = it % STAGES;
-          if (it >= STAGES && !mbar_wait(empty + st, (it / STAGES - 1) & 1, abort_flag, kErrFp8)) { ok = false; break; }
-          unsigned char* s = smem + st * S::kStage;
-          mbar_expect_tx(full + st, S::kStage);
-          tma_load_2d(s, &tm_x, kb * 128, m0, full + st);
-          tma_load_2d(s + S::kA, &tm_w, kb * 128, n0, full + st);
-        }
-      }
-      // every load that was issued has landed before the shared memory is given up
-      for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_drain(full + i % STAGES, (i / STAGES) & 1);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t id = idesc_e4m3(BN);
-      int it = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
-        for (int kb = 0; kb < a.kb; ++kb, ++it) {
-          const int st = it % STAGES, buf = it & 1;
-          if (!mbar_wait(full + st, (it / STAGES) & 1, abort_flag, kErrFp8 + 1) ||
-              (it >= 2 && !mbar_wait(d_empty + buf, (it / 2 - 1) & 1, abort_flag, kErrFp8 + 2))) {
-            ok = false;
-            break;
+          if (it >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(done + st, phase, abort_flag, kErrFp8));
+          if (!ok) break;
+          if (leader) {
+            unsigned char* s = smem + st * S::kStage;
+            if (rank == 0) mbar_expect_tx(full + st, S::kStage * PAIR);
+            if constexpr (PAIR == 2) {
+              const uint32_t bar = peer_addr(full + st, 0);
+              tma_load_2d_pair(s, &tm_x, kb * 128, m0, bar);
+              tma_load_2d_pair(s + S::kA, &tm_w, kb * 128, n0, bar);
+            } else {
+              tma_load_2d(s, &tm_x, kb * 128, m0, full + st);
+              tma_load_2d(s + S::kA, &tm_w, kb * 128, n0, full + st);
+            }
           }
-          fence_after();
-          const uint32_t xa = smem_u32(smem + st * S::kStage), wa = xa + S::kA;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ss_f8(tmem + buf * BN, sdesc(xa + k * 32, 16, 1024), sdesc(wa + k * 32, 16, 1024), id, k != 0);
-          mma_commit(empty + st);
-          mma_commit(d_full + buf);
+          __syncwarp();
+          if (++st == STAGES) { st = 0; phase ^= 1; }
         }
       }
-      mma_commit(drain);
-      mbar_drain(drain, 0);
+      // every load that was issued has landed before the shared memory is given up (the even CTA's barriers
+      // count both CTAs' bytes, and no CTA leaves before the cluster's last barrier)
+      if (rank == 0 && leader)
+        for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_drain(full + i % STAGES, (i / STAGES) & 1);
+    }
+    if (warp == 1 && rank == 0) {
+      constexpr uint32_t id = idesc_e4m3(BN, 128 * PAIR);
+      const uint64_t dx0 = sdesc(smem_u32(smem), 16, 1024), dw0 = sdesc(smem_u32(smem) + S::kA, 16, 1024);
+      int st = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = group; tile < a.tiles && ok; tile += groups) {
+        for (int kb = 0; kb < a.kb; ++kb, ++it) {
+          const int buf = it & 1;
+          if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(d_empty + buf, (it / 2 - 1) & 1, abort_flag, kErrFp8 + 2));
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(full + st, phase, abort_flag, kErrFp8 + 1));
+          if (!ok) break;
+          fence_after();
+          const uint64_t dx = dx0 + (uint64_t)(st * (S::kStage >> 4)), dw = dw0 + (uint64_t)(st * (S::kStage >> 4));
+          const uint32_t d = tmem + buf * BN;
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // 32 bytes along the channels: 2 in the descriptor's 16-byte units
+              if constexpr (PAIR == 2) mma_ss_f8_pair(d, dx + 2 * k, dw + 2 * k, id, k != 0);
+              else mma_ss_f8(d, dx + 2 * k, dw + 2 * k, id, k != 0);
+            }
+            if constexpr (PAIR == 2) mma_commit_pair(done + st, 3); else mma_commit(done + st);
+          }
+          __syncwarp();
+          if (++st == STAGES) { st = 0; phase ^= 1; }
+        }
+      }
+      if (leader) {
+        if constexpr (PAIR == 2) mma_commit_pair(drain, 1); else mma_commit(drain);
+        mbar_drain(drain, 0);
+      }
     }
   } else {
-    constexpr int COLS = BN / 2;                // columns of this warp
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    constexpr int COLS = BN / 2;  // columns of this warp
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    unsigned char* stage = smem + S::kOut + (warp - 2) * 4096;
-    int it = 0;
+    unsigned char* stage = smem + S::kOut + (warp - 4) * 4096;
+    const uint32_t free0 = peer_addr(d_empty, 0);
+    int it = 0, st = 0;
+    uint32_t phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
-      const int m0 = tile / a.tiles_n * 128 + quarter * 32, n0 = tile % a.tiles_n * BN + half * COLS;
+    for (int tile = group; tile < a.tiles && ok; tile += groups) {
+      const int m0 = tile / a.tiles_n * (128 * PAIR) + rank * 128 + quarter * 32, n0 = tile % a.tiles_n * BN + part * COLS;
       const int row = m0 + lane;
-      const float* xs = a.xs + (int64_t)(row < a.m ? row : a.m - 1) * a.kb;
+      const float* xs = a.xs + (int64_t)(row < a.m ? row : a.m - 1) * a.xs_stride;
       const float* ws = a.ws + (int64_t)((n0 < a.n ? n0 : a.n - 1) / 128) * a.ws_stride;
       uint64_t acc[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; ++i) acc[i] = 0ull;
-      float s_next = xs[0] * ws[0];
+      // the scales of four blocks at a time, loaded four blocks before they are multiplied: with nearly all of
+      // the SM's memory taken as shared memory they come from L2, and a distance of one block was too short
+      float4 xn = scales4(xs, 0, a.kb, a.xs_vec), wn = scales4(ws, 0, a.kb, false), s4 = xn;
       for (int kb = 0; kb < a.kb; ++kb, ++it) {
         const int buf = it & 1;
-        const float s = s_next;
-        if (kb + 1 < a.kb) s_next = xs[kb + 1] * ws[kb + 1];
-        const uint64_t s2 = pack2(s, s);
-        ok = __all_sync(0xffffffffu, mbar_wait(d_full + buf, (it / 2) & 1, abort_flag, kErrFp8 + 3));
+        if ((kb & 3) == 0) {
+          s4 = make_float4(xn.x * wn.x, xn.y * wn.y, xn.z * wn.z, xn.w * wn.w);
+          xn = scales4(xs, kb + 4, a.kb, a.xs_vec);
+          wn = scales4(ws, kb + 4, a.kb, false);
+        }
+        const uint64_t s2 = f32x2(s4.x, s4.x);
+        s4 = make_float4(s4.y, s4.z, s4.w, s4.x);
+        ok = __all_sync(0xffffffffu, mbar_wait(done + st, phase, abort_flag, kErrFp8 + 3));
         if (!ok) break;
+        if (++st == STAGES) { st = 0; phase ^= 1; }
         fence_after();
+        const uint32_t at = tmem + lane_addr + buf * BN + part * COLS;
 #pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-          uint32_t r[32];
-          HGA_LD32(tmem + lane_addr + buf * BN + half * COLS + c, r);
+        for (int c = 0; c < COLS; c += 64) {
+          uint32_t r[2][32];  // two reads under way together
+          HGA_LD32(at + c, r[0]);
+          HGA_LD32(at + c + 32, r[1]);
           tmem_wait_ld();
-          if (c + 32 == COLS) {
+          if (c + 64 == COLS) {
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(d_empty + buf);
+            if (lane == 0) {
+              if constexpr (PAIR == 2) mbar_arrive_peer(free0 + 8 * buf); else mbar_arrive(d_empty + buf);
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            acc[c / 2 + i] = ffma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s2, acc[c / 2 + i]);
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              acc[c / 2 + h * 16 + i] = f32x2_fma(f32x2(__uint_as_float(r[h][2 * i]), __uint_as_float(r[h][2 * i + 1])), s2,
+                                                  acc[c / 2 + h * 16 + i]);
         }
       }
       if (!ok) break;
@@ -214,7 +279,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float lo, hi;
-              unpack2(acc[c / 2 + j * 4 + e], lo, hi);
+              f32x2_get(acc[c / 2 + j * 4 + e], lo, hi);
               if (bias) {
                 const int col = n0 + c + j * 8 + e * 2;
                 lo += col < a.n ? Num<T>::to_f(bias[col]) : 0.f;
@@ -226,7 +291,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float lo, hi;
-              unpack2(acc[c / 2 + j * 2 + e], lo, hi);
+              f32x2_get(acc[c / 2 + j * 2 + e], lo, hi);
               if (bias) {
                 const int col = n0 + c + j * 4 + e * 2;
                 lo += col < a.n ? Num<T>::to_f(bias[col]) : 0.f;
@@ -260,18 +325,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   fence_before();
   __syncthreads();
+  if constexpr (PAIR == 2) cluster_sync();  // the pair's MMAs read both CTAs' shared memory and write both TMEMs
   fence_after();
-  if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * BN));
+  if (warp == 1) {
+    if constexpr (PAIR == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * BN));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * BN));
+  }
 }
 
-template <typename T, int BN, int STAGES>
-static cudaError_t tiles_t(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                           int64_t w_stride, cudaStream_t st) {
+template <typename T, int BN, int PAIR, int STAGES>
+static cudaError_t tiles_t(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                           const void* w, int64_t w_stride, cudaStream_t st) {
   CUtensorMap mx, mw, mo;
   const cuuint64_t dx[2] = {(cuuint64_t)a.k, (cuuint64_t)a.m}, sx[1] = {(cuuint64_t)q_stride};
   const cuuint64_t dw[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n}, sw[1] = {(cuuint64_t)w_stride};
-  const cuuint32_t bx[2] = {128, 128}, bw[2] = {128, BN};
+  const cuuint32_t bx[2] = {128, 128}, bw[2] = {128, BN / PAIR};
   if (!make_map_typed(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, 2, dx, sx, bx, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_map_typed(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, 2, dw, sw, bw, CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
@@ -287,38 +357,48 @@ static cudaError_t tiles_t(const Fp8Linear& a, const void* q, int64_t q_stride, 
   TileArgs t;
   t.m = (int)a.m; t.n = (int)a.n; t.kb = (int)((a.k + 127) / 128);
   t.tiles_n = (int)((a.n + BN - 1) / BN);
-  const int64_t tiles = (a.m + 127) / 128 * t.tiles_n;
+  const int64_t tiles = (a.m + 128 * PAIR - 1) / (128 * PAIR) * t.tiles_n;
   if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
   t.tiles = (int)tiles;
-  t.xs = xs; t.ws = a.w_scale; t.ws_stride = a.ws_stride;
+  t.xs = xs; t.xs_stride = xs_stride; t.xs_vec = xs_stride % 4 == 0 && ((uintptr_t)xs & 15) == 0 && xs_stride >= (t.kb + 3) / 4 * 4; t.ws = a.w_scale; t.ws_stride = a.ws_stride;
   t.bias = a.bias; t.out = a.out; t.out_stride = a.out_stride; t.tma_out = tma_out;
-  constexpr int smem = TileSmem<BN, STAGES>::kTotal + 1024;
-  auto kern = fp8_tiles_kernel<T, BN, STAGES>;
+  constexpr int smem = TileSmem<BN, PAIR, STAGES>::kTotal + 1024;
+  auto kern = fp8_tiles_kernel<T, BN, PAIR, STAGES>;
   static unsigned long long raised = 0;
   cudaError_t e = raise_smem_limit((const void*)kern, smem, &raised);
   if (e != cudaSuccess) return e;
-  kern<<<t.tiles < 148 ? t.tiles : 148, kTileThreads, smem, st>>>(mx, mw, mo, t);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((t.tiles < 148 / PAIR ? t.tiles : 148 / PAIR) * PAIR);
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, mx, mw, mo, t);
 }
 
 template <typename T>
-static cudaError_t tiles_n(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                           int64_t w_stride, cudaStream_t st) {
-  // 128 x 256 tiles read the operands from shared memory fewer times; where they would leave SMs
-  // without a tile, 128 x 128 ones
-  const int64_t rows = (a.m + 127) / 128;
-  if (rows * ((a.n + 255) / 256) >= 148) return tiles_t<T, 256, 4>(a, q, q_stride, xs, w, w_stride, st);
-  return tiles_t<T, 128, 5>(a, q, q_stride, xs, w, w_stride, st);
+static cudaError_t tiles_n(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                           const void* w, int64_t w_stride, cudaStream_t st) {
+  // 256 x 256 tiles of CTA pairs where they fill the GPU: a pair reads half as many bytes per product as
+  // 128 x 128 tiles, and the loads from L2 are what bounds them
+  const int64_t pairs = (a.m + 255) / 256 * ((a.n + 255) / 256);
+  if (pairs >= 74) return tiles_t<T, 256, 2, 6>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  return tiles_t<T, 128, 1, 5>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
 }
 
 }  // namespace tc
 
-cudaError_t launch_fp8_tiles(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, const void* w,
-                             int64_t w_stride, cudaStream_t st) {
+cudaError_t launch_fp8_tiles(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
+                             const void* w, int64_t w_stride, cudaStream_t st) {
   switch (a.out_dtype) {
-    case HGA_DTYPE_F32: return tc::tiles_n<float>(a, q, q_stride, xs, w, w_stride, st);
-    case HGA_DTYPE_BF16: return tc::tiles_n<__nv_bfloat16>(a, q, q_stride, xs, w, w_stride, st);
-    case HGA_DTYPE_F16: return tc::tiles_n<__half>(a, q, q_stride, xs, w, w_stride, st);
+    case HGA_DTYPE_F32: return tc::tiles_n<float>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+    case HGA_DTYPE_BF16: return tc::tiles_n<__nv_bfloat16>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+    case HGA_DTYPE_F16: return tc::tiles_n<__half>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
   }
   return cudaErrorInvalidValue;
 }

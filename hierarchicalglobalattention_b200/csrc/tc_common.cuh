@@ -65,19 +65,25 @@ __device__ __forceinline__ unsigned long long global_ns() {
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code,
                                           unsigned long long limit_ns = kWaitLimitNs) {
-  if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = global_ns();
-  // try_wait may suspend the thread for a hardware-defined time: check the clock and the CTA's
-  // abort flag after every attempt so the limit holds regardless of that time
-  while (!mbar_try(bar, parity)) {
+  // The clock is looked at once in 64 attempts, and not before the first 64: reading %globaltimer takes
+  // several hundred cycles, which every wait that was not ready at once used to pay.  An attempt suspends the
+  // thread for a hardware-defined time of at most about 20 us, so the limit holds within a few milliseconds;
+  // the CTA's abort flag is checked after every attempt.
+  unsigned long long t0 = 0;
+  for (int i = 1;; ++i) {
+    if (mbar_try(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (global_ns() - t0 > limit_ns) {
-      *abort_flag = 1;
-      atomicCAS(&g_tc_error, 0, code);
-      return false;
+    if ((i & 63) == 0) {
+      const unsigned long long t = global_ns();
+      if (t0 == 0) {
+        t0 = t;
+      } else if (t - t0 > limit_ns) {
+        *abort_flag = 1;
+        atomicCAS(&g_tc_error, 0, code);
+        return false;
+      }
     }
   }
-  return true;
 }
 
 // Bounded wait that ignores the CTA abort flag: used on the way out, to let copies and MMAs that
@@ -149,9 +155,46 @@ __device__ __forceinline__ void mma_ss_f8(uint32_t d_tmem, uint64_t a, uint64_t 
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-// Instruction descriptor: e4m3 x e4m3 -> f32, both K-major, M = 128.
-__host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t n) {
-  return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+// The same for a pair of CTAs: A and D rows 0-127 are the even CTA's, 128-255 the odd one's, each holds half
+// of B's rows; issued by the even CTA.
+__device__ __forceinline__ void mma_ss_f8_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// Instruction descriptor: e4m3 x e4m3 -> f32, both K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t n, uint32_t m = 128) {
+  return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+// Completion of the pair's MMAs so far on the barrier at this offset in the CTAs of `mask`.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint16_t mask) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(mask)
+      : "memory");
+}
+// The address of the same shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+// An arrival on another CTA's barrier.  Cluster-scope release here and acquire at the waiting side compile to
+// memory barriers that wait for every outstanding access (they took two thirds of the pair kernel's time);
+// what is ordered is TMEM traffic, by tcgen05.wait::ld and the tcgen05 fences on both sides.
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// A tile load of one CTA of a pair whose bytes are counted on a barrier of either CTA (a cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))

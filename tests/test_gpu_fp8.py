@@ -97,6 +97,21 @@ def test_linear(cuda, M, N, K, dtype):
     _check(y, xq, xs, w, ws, bias, dtype)
 
 
+@pytest.mark.parametrize("M,N,K,dtype", [(2500, 2000, 300, torch.bfloat16), (4900, 1024, 64, torch.float16),
+                                         (5001, 1111, 1000, torch.bfloat16), (9500, 512, 640, torch.float32),
+                                         (257, 19000, 272, torch.bfloat16), (20000, 300, 128, torch.float16)])
+def test_linear_many_tiles(cuda, M, N, K, dtype):
+    """Products that fill the GPU with tiles, whole and ragged in every direction."""
+    from hierarchicalglobalattention_b200 import ops
+    g = torch.Generator().manual_seed(M)
+    x = _x(g, M, K, dtype)
+    w, ws = _weight(g, N, K)
+    bias = torch.randn(N, generator=g).to(dtype) if N % 2 else None
+    y = ops.fp8_linear(x.to(cuda), w.to(cuda), ws.to(cuda), bias=None if bias is None else bias.to(cuda))
+    xq, xs = R.fp8_quantize(x)
+    _check(y, xq, xs, w, ws, bias, dtype)
+
+
 @pytest.mark.parametrize("M", [1, 9, 40, 300])
 def test_linear_quantised_input(cuda, M):
     """8-bit rows with their scales give what the same rows give when they are quantised on the way in."""
