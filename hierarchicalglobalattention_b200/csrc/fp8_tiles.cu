@@ -13,7 +13,7 @@
 //   warp 1      MMA issuer (of the even CTA), TMEM owner
 //   warps 4-11  each reads 32 TMEM lanes (rows) x BN / 2 columns: one row a thread, one weight block a
 //               warp, so a block's scale is one product per thread
-// Results go through 4 KB of swizzled shared memory per warp to whole-line TMA stores (plain stores where
+// Results go through two 4 KB pieces of swizzled shared memory per warp to whole-line TMA stores (plain stores where
 // the output's rows are off the 16-byte grid).  Waits are bounded as in tc_common.cuh.
 #include "fp8_common.cuh"
 #include "tc_common.cuh"
@@ -54,8 +54,8 @@ __device__ __forceinline__ float4 scales4(const float* p, int kb, int n, bool ve
 template <int BN, int PAIR, int STAGES> struct TileSmem {
   static constexpr int kA = 128 * 128, kB = BN / PAIR * 128;
   static constexpr int kStage = kA + kB;
-  static constexpr int kOut = STAGES * kStage;       // 4 KB per epilogue warp
-  static constexpr int kBars = kOut + kEpiWarps * 4096;
+  static constexpr int kOut = STAGES * kStage;       // 2 x 4 KB per epilogue warp
+  static constexpr int kBars = kOut + kEpiWarps * 8192;
   static constexpr int kMisc = kBars + (2 * STAGES + 3) * 8;
   static constexpr int kTotal = kMisc + 32;
 };
@@ -66,7 +66,7 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // One lane of the warp, the same one every time; all lanes call.
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int COLS = BN / 2;  // columns of this warp
     const int quarter = warp & 3, part = (warp - 4) >> 2;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    unsigned char* stage = smem + S::kOut + (warp - 4) * 4096;
+    unsigned char* stage = smem + S::kOut + (warp - 4) * 8192;
     const uint32_t free0 = peer_addr(d_empty, 0);
     int it = 0, st = 0;
     uint32_t phase = 0;
@@ -268,8 +268,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int c = 0; c < COLS; c += PC) {
         if (n0 + c >= a.n || m0 >= a.m) break;  // warp-uniform
+        unsigned char* stg = stage + ((c / PC) & 1) * 4096;
         if (a.tma_out) {
-          if (lane == 0) bulk_wait_read();
+          if (lane == 0) bulk_wait_read1();  // the store before the last has been read out
           __syncwarp();
         }
 #pragma unroll
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
           }
           if (a.tma_out) {
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           } else if (row < a.m) {
             T* o = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + n0 + c + j * (16 / (int)sizeof(T));
             const T* v = reinterpret_cast<const T*>(w);
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tm_o, stage, n0 + c, m0);
+            tma_store_2d(&tm_o, stg, n0 + c, m0);
             bulk_commit();
           }
         }
@@ -387,8 +388,8 @@ static cudaError_t tiles_n(const Fp8Linear& a, const void* q, int64_t q_stride, 
   // 256 x 256 tiles of CTA pairs where they fill the GPU: a pair reads half as many bytes per product as
   // 128 x 128 tiles, and the loads from L2 are what bounds them
   const int64_t pairs = (a.m + 255) / 256 * ((a.n + 255) / 256);
-  if (pairs >= 74) return tiles_t<T, 256, 2, 6>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
-  return tiles_t<T, 128, 1, 5>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  if (pairs >= 74) return tiles_t<T, 256, 2, 5>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  return tiles_t<T, 128, 1, 4>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
 }
 
 }  // namespace tc
