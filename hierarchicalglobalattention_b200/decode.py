@@ -32,6 +32,11 @@ class DecodeContext:
 
     def attend(self, q: torch.Tensor) -> torch.Tensor:
         store = self.router.store
+        if getattr(store, "kv_bits", 16) == 4:
+            out = store.attend_decode(self.layer, self.params, q, self.seq_pos, self.routing["open_gid"],
+                                      self.routing["open_t0"])
+            self.finish()
+            return out
         hot_k, hot_v = store.hot_buffers(self.layer)
         cold_k, cold_v = store.cold_buffers(self.layer)
         open_gid = self.routing["open_gid"]
@@ -49,6 +54,8 @@ class DecodeContext:
         """Dual Chunk Attention of the block (qwen_routed_attention.py:247-283): q_raw [B,H,L,Dh]
         before RoPE; the store holds keys roped at their intra-chunk positions."""
         store = self.router.store
+        if getattr(store, "kv_bits", 16) == 4:
+            raise NotImplementedError("Dual Chunk Attention reads the 16-bit record; use a 16-bit store")
         hot_k, hot_v = store.hot_buffers(self.layer)
         cold_k, cold_v = store.cold_buffers(self.layer)
         open_gid = open_pos = self.routing["open_gid"]

@@ -68,8 +68,14 @@ class DecodeStepGraph:
                               store.hot_mode, None if store.hot_mode == 0 else cold_k,
                               None if store.hot_mode == 0 else cold_v, store.active_raw(layer))
             r = ops.route_decode(self.hp, self.q[i], self.seq_pos, st.chunk_k, st.group_k, self.nmid)
-            ops.attend_decode(self.hp, self.q[i], self.seq_pos, hot_k, hot_v, store.hot_mode, cold_k, cold_v,
-                              r["open_gid"], r["open_t0"], out=self.out[i])
+            if getattr(store, "kv_bits", 16) == 4:
+                # the record is read in place (the bank's stamps advance on the host, outside a graph)
+                rec_k, rec_v = store.record(layer)
+                ops.attend_decode_kv4(self.hp, self.q[i], self.seq_pos, hot_k, hot_v, rec_k, rec_v, r["open_gid"],
+                                      r["open_t0"], out=self.out[i])
+            else:
+                ops.attend_decode(self.hp, self.q[i], self.seq_pos, hot_k, hot_v, store.hot_mode, cold_k, cold_v,
+                                  r["open_gid"], r["open_t0"], out=self.out[i])
         self.seq_pos.add_(1)
 
     def _capture(self) -> None:

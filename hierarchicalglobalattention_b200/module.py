@@ -8,6 +8,8 @@ state_dicts load unchanged), forward signature, return value ``(out, {})`` and r
   one fused QKV projection GEMM (cuBLAS via torch)  ->  hga_qkv_prologue (RMSNorm + RoPE + store
   layout)  ->  ChunkRouter (summary builder, two-level router / incremental decode kernels)  ->
   working-set attention kernel writing [B,S,H,Dh]  ->  o_proj GEMM.
+
+``kv_bits=4`` (no counterpart in the reference) keeps the cold token record in 4 bits (``Kv4CacheStore``).
 """
 from __future__ import annotations
 
@@ -81,8 +83,11 @@ class HierarchicalGlobalAttentionRouted(nn.Module):
                  topk_chunks: int = 20, topk_groups: int = 32, keep_first: int = 1, keep_last: int = 2,
                  head_dim: Optional[int] = None, qk_norm: bool = False, norm_eps: float = 1e-6,
                  theta: float = 1_000_000.0, layer_idx: int = 0, cache_location: str = "vram",
-                 num_layers: int = 0, **kwargs: Any) -> None:
+                 num_layers: int = 0, kv_bits: int = 16, **kwargs: Any) -> None:
         super().__init__()
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 (the model's type) or 4; got {kv_bits}")
+        self.kv_bits = int(kv_bits)
         assert nhead % kv_heads == 0
         head_dim = d_model // nhead if head_dim is None else head_dim
         self.d_model, self.nhead, self.kv_heads, self.head_dim = d_model, nhead, kv_heads, head_dim
@@ -150,6 +155,10 @@ class HierarchicalGlobalAttentionRouted(nn.Module):
         kwargs = dict(compute_device=device, policy=self._policy, kv_heads=self.kv_heads, head_dim=self.head_dim,
                       chunk_size=self.chunk_size, groups_per_chunk=self._cfg.groups_per_chunk, batch_size=B,
                       dtype=dtype)
+        if self.kv_bits == 4:
+            from .store_kv4 import Kv4CacheStore
+            return Kv4CacheStore(record_device="cuda" if self.cache_location == "vram" else "cpu",
+                                 num_layers=self.num_layers, **kwargs)
         if self.cache_location == "vram":
             return VramKVCacheStore(**kwargs)
         from .store_ram import RamKVCacheStore

@@ -18,7 +18,12 @@ concatenated QKV projection GEMM.  RoPE theta is read from ``config.rope_paramet
 Dual Chunk Attention (``dca_chunk > 0``, qwen_routed_attention.py:210-283): keys stored roped at
 their intra-chunk position ``pos % dca_chunk``, routed with intra-roped queries through the
 incremental path, attended by the DCA decode kernel (three fp32 ropings of each query chosen per
-key by DCA chunk).  Not carried over: the file-system cache tier (``cache_location="fs"``), which
+key by DCA chunk).
+
+Low-bit layers (no counterpart in the reference): ``kv_bits=4`` keeps the cold token record in 4 bits
+(``Kv4CacheStore``: in HBM for cache_location "vram", in pinned host memory for "ram"), and
+``fp8_projections=True`` runs the q/k/v and output projections as 8-bit block-scaled products - the layers of
+an FP8 checkpoint as they are, plain linear layers quantised once.  Not carried over: the file-system cache tier (``cache_location="fs"``), which
 raises.
 """
 from __future__ import annotations
@@ -31,6 +36,7 @@ import torch.nn.functional as F
 
 from .config import ChunkPlacementPolicy, RouterConfig
 from . import ops
+from .fp8 import fp8_concat
 from .module import routed_attention
 from .router import ChunkRouter
 from .store import VramKVCacheStore
@@ -91,8 +97,13 @@ class QwenRoutedAttention(nn.Module):
                  keep_first: int = 2, keep_last: int = 2, topk_chunks: int = 8, topk_groups: int = 32,
                  cache_location: str = "vram", vram_cache_chunks: int = 256, vram_summary_chunks: int = 4096,
                  vram_cache_reserve_gb: float = 1.5, ram_budget_gb: float = 12.0,
-                 fs_cache_dir: Optional[str] = None, dca_chunk: int = 0, dca_local: int = 0) -> None:
+                 fs_cache_dir: Optional[str] = None, dca_chunk: int = 0, dca_local: int = 0, kv_bits: int = 16,
+                 fp8_projections: bool = False) -> None:
         super().__init__()
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 (the model's type) or 4; got {kv_bits}")
+        if kv_bits == 4 and dca_chunk > 0:
+            raise ValueError("Dual Chunk Attention reads the 16-bit record: kv_bits=4 goes with dca_chunk=0")
         if cache_location not in ("vram", "ram"):
             raise NotImplementedError(f"cache_location={cache_location!r}: the B200 path provides 'vram' and 'ram'")
         self.orig = orig
@@ -109,6 +120,8 @@ class QwenRoutedAttention(nn.Module):
         self.vram_cache_reserve_gb = vram_cache_reserve_gb
         self.ram_budget_gb = ram_budget_gb
         self.fs_cache_dir = fs_cache_dir
+        self.kv_bits = int(kv_bits)
+        self.fp8_projections = bool(fp8_projections)
         if dca_chunk > 0 and dca_chunk % chunk_size != 0:
             # a routing chunk must lie inside one DCA chunk (qwen_routed_attention.py:137-141)
             raise ValueError(f"dca_chunk ({dca_chunk}) must be a multiple of chunk_size ({chunk_size})")
@@ -121,6 +134,7 @@ class QwenRoutedAttention(nn.Module):
                                  topk_groups=topk_groups, theta=rope_theta_of(config))
         self._policy = ChunkPlacementPolicy(keep_last=keep_last, keep_first=keep_first, first_token_level=True)
         self._qkv_cache = None
+        self._fp8_cache: dict = {}
 
     # ------------------------------------------------------------------------------------------
     def _qkv(self, x: torch.Tensor) -> torch.Tensor:
@@ -128,6 +142,8 @@ class QwenRoutedAttention(nn.Module):
         projections are plain ``nn.Linear`` layers, else the three modules' outputs concatenated."""
         o = self.orig
         projs = (o.q_proj, o.k_proj, o.v_proj)
+        if self.fp8_projections:
+            return self._fp8(x, "qkv", projs)
         if all(type(m) is nn.Linear for m in projs):
             ps = tuple(m.weight for m in projs) + tuple(m.bias for m in projs)
             key = tuple((t.data_ptr(), t._version, t.dtype) if t is not None else None for t in ps)
@@ -140,6 +156,27 @@ class QwenRoutedAttention(nn.Module):
                 self._qkv_cache = (key, w, b)
             return F.linear(x, self._qkv_cache[1], self._qkv_cache[2])
         return torch.cat([m(x) for m in projs], dim=-1).contiguous()
+
+    def _fp8(self, x: torch.Tensor, name: str, mods) -> torch.Tensor:
+        """The layers' outputs on x, side by side, as 8-bit block-scaled products: one for all of them when
+        their blocks line up.  Layers of an FP8 checkpoint are used as they are; plain linear layers are
+        quantised once (again when a weight changes)."""
+        ts = tuple(m.weight for m in mods) + tuple(getattr(m, "weight_scale_inv", None) for m in mods) + tuple(
+            getattr(m, "bias", None) for m in mods)
+        key = tuple((t.data_ptr(), t._version, t.dtype) if t is not None else None for t in ts)
+        hit = self._fp8_cache.get(name)
+        if hit is None or hit[0] != key:
+            whole = fp8_concat(mods)
+            parts = [whole] if whole is not None else [fp8_concat([m]) for m in mods]
+            if any(p is None for p in parts):
+                raise TypeError("fp8_projections needs nn.Linear layers or 8-bit layers with 128 x 128 block scales")
+            hit = (key, parts)
+            self._fp8_cache[name] = hit
+        ys = [ops.fp8_linear(x, w, s, bias=None if b is None else b.to(x.dtype)) for w, s, b in hit[1]]
+        return ys[0] if len(ys) == 1 else torch.cat(ys, dim=-1)
+
+    def _o_proj(self, heads: torch.Tensor) -> torch.Tensor:
+        return self._fp8(heads, "o", (self.orig.o_proj,)) if self.fp8_projections else self.orig.o_proj(heads)
 
     def forward(self, hidden_states: torch.Tensor, position_embeddings: Tuple[torch.Tensor, torch.Tensor],
                 attention_mask: Optional[torch.Tensor] = None, past_key_values: Any = None,
@@ -171,7 +208,7 @@ class QwenRoutedAttention(nn.Module):
         eps = float(getattr(o.q_norm, "variance_epsilon", getattr(o.q_norm, "eps", 1e-6)))
         out_heads = routed_attention(router, self.layer_idx, hp, qkv, cos, sin, start_pos, start_pos, qn, kn, eps,
                                      norm_mode=1, rope_mode=1, round_table=False)
-        return o.o_proj(out_heads.view(B, S, H * Dh)), None
+        return self._o_proj(out_heads.view(B, S, H * Dh)), None
 
     # ------------------------------------------------------------------------------------------
     def _dca_forward(self, x: torch.Tensor, start_pos: int, router: ChunkRouter) -> torch.Tensor:
@@ -208,13 +245,18 @@ class QwenRoutedAttention(nn.Module):
             out_heads[:, sl] = rk.attend_dca(q_raw[:, :, sl], pos[sl], L_c, self.dca_ceil, theta).transpose(1, 2)
             p += take
             done += take
-        return o.o_proj(out_heads.view(B, S, H * Dh))
+        return self._o_proj(out_heads.view(B, S, H * Dh))
 
     # ------------------------------------------------------------------------------------------
     def _make_store(self, B: int, dtype: torch.dtype, device: torch.device):
         kwargs = dict(compute_device=device, policy=self._policy, kv_heads=self.num_kv_heads, head_dim=self.head_dim,
                       chunk_size=self.chunk_size, groups_per_chunk=self._cfg.groups_per_chunk, batch_size=B,
                       dtype=dtype)
+        if self.kv_bits == 4:
+            from .store_kv4 import Kv4CacheStore
+            return Kv4CacheStore(record_device="cuda" if self.cache_location == "vram" else "cpu",
+                                 vram_cache_chunks=self.vram_cache_chunks, vram_summary_chunks=self.vram_summary_chunks,
+                                 num_layers=self.num_layers, vram_cache_reserve_gb=self.vram_cache_reserve_gb, **kwargs)
         if self.cache_location == "vram":
             return VramKVCacheStore(**kwargs)
         from .store_ram import RamKVCacheStore
@@ -257,7 +299,7 @@ def replace_qwen_attention_with_router(model: nn.Module, *, keep_first: int = 2,
                                        vram_cache_chunks: int = 256, vram_summary_chunks: int = 4096,
                                        vram_cache_reserve_gb: float = 1.5, ram_budget_gb: float = 12.0,
                                        fs_cache_dir: Optional[str] = None, dca_chunk: int = 0,
-                                       dca_local: int = 0) -> int:
+                                       dca_local: int = 0, kv_bits: int = 16, fp8_projections: bool = False) -> int:
     """Replace every decoder layer's ``self_attn`` with a ``QwenRoutedAttention`` (idempotent:
     earlier replacements are undone first).  Returns the number of layers replaced."""
     restore_original_attention(model)
@@ -269,7 +311,7 @@ def replace_qwen_attention_with_router(model: nn.Module, *, keep_first: int = 2,
             keep_last=keep_last, topk_chunks=topk_chunks, topk_groups=topk_groups, cache_location=cache_location,
             vram_cache_chunks=vram_cache_chunks, vram_summary_chunks=vram_summary_chunks,
             vram_cache_reserve_gb=vram_cache_reserve_gb, ram_budget_gb=ram_budget_gb, fs_cache_dir=fs_cache_dir,
-            dca_chunk=dca_chunk, dca_local=dca_local)
+            dca_chunk=dca_chunk, dca_local=dca_local, kv_bits=kv_bits, fp8_projections=fp8_projections)
         count += 1
     return count
 

@@ -15,6 +15,11 @@ Operators (the C entry point each wraps):
   hga::attend_decode  (hga_attend_decode)    -> out [B,H,L,Dh]
   hga::attend_decode_dca (hga_attend_decode_dca) -> out [B,H,L,Dh]
   hga::gather_h2d     (hga_gather_h2d)       -> open_slot (mutates the bank and its maps)
+  hga::fp8_quantize   (hga_fp8_quantize)     -> q, scale
+  hga::fp8_linear     (hga_fp8_linear)       -> y [..., N]
+  hga::kv4_pack       (hga_kv4_pack)         -> rec_k, rec_v
+  hga::kv4_unpack     (hga_kv4_unpack)       -> k, v
+  hga::attend_decode_kv4 (hga_attend_decode_kv4) -> out [B,H,L,Dh]
 """
 from __future__ import annotations
 
@@ -141,3 +146,62 @@ def gather_h2d(pi: List[int], pf: List[float], open_gid: Tensor, rec_k: Tensor, 
 @gather_h2d.register_fake
 def _(pi, pf, open_gid, rec_k, rec_v, bank_k, bank_v, slot_gid, gid_slot, slot_stamp, stamp, counters):
     return torch.empty_like(open_gid)
+
+
+# ---- 8-bit products and the 4-bit record ------------------------------------------------------
+@torch.library.custom_op("hga::fp8_quantize", mutates_args=())
+def fp8_quantize(x: Tensor) -> Tuple[Tensor, Tensor]:
+    return ops.fp8_quantize(x)
+
+
+@fp8_quantize.register_fake
+def _(x):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty((*x.shape[:-1], -(-x.shape[-1] // ops.FP8_BLOCK)), dtype=torch.float32))
+
+
+@torch.library.custom_op("hga::fp8_linear", mutates_args=())
+def fp8_linear(x: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor], x_scale: Optional[Tensor],
+               out_dtype: Optional[torch.dtype]) -> Tensor:
+    return ops.fp8_linear(x, w, w_scale, bias=bias, x_scale=x_scale, out_dtype=out_dtype)
+
+
+@fp8_linear.register_fake
+def _(x, w, w_scale, bias, x_scale, out_dtype):
+    dt = out_dtype or (torch.bfloat16 if x.dtype == torch.float8_e4m3fn else x.dtype)
+    return x.new_empty((*x.shape[:-1], w.shape[0]), dtype=dt)
+
+
+@torch.library.custom_op("hga::kv4_pack", mutates_args=())
+def kv4_pack(k: Tensor, v: Tensor) -> Tuple[Tensor, Tensor]:
+    return ops.kv4_pack(k, v)
+
+
+@kv4_pack.register_fake
+def _(k, v):
+    B, KVH, S, Dh = k.shape
+    shape = (B, KVH, -(-S // ops.KV4_UNIT), ops.kv4_unit_bytes(Dh))
+    return k.new_empty(shape, dtype=torch.uint8), k.new_empty(shape, dtype=torch.uint8)
+
+
+@torch.library.custom_op("hga::kv4_unpack", mutates_args=())
+def kv4_unpack(rec_k: Tensor, rec_v: Tensor, seq_len: int, dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    return ops.kv4_unpack(rec_k, rec_v, seq_len, dtype)
+
+
+@kv4_unpack.register_fake
+def _(rec_k, rec_v, seq_len, dtype):
+    B, KVH, _, nb = rec_k.shape
+    shape = (B, KVH, seq_len, nb // 10)
+    return rec_k.new_empty(shape, dtype=dtype), rec_k.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("hga::attend_decode_kv4", mutates_args=())
+def attend_decode_kv4(pi: List[int], pf: List[float], q: Tensor, seq_pos: Tensor, hot_k: Tensor, hot_v: Tensor,
+                      rec_k: Tensor, rec_v: Tensor, open_gid: Tensor, open_t0: Tensor) -> Tensor:
+    return ops.attend_decode_kv4(_params(pi, pf), q, seq_pos, hot_k, hot_v, rec_k, rec_v, open_gid, open_t0)
+
+
+@attend_decode_kv4.register_fake
+def _(pi, pf, q, seq_pos, hot_k, hot_v, rec_k, rec_v, open_gid, open_t0):
+    return torch.empty_like(q)

@@ -81,3 +81,60 @@ def test_weight_quantisation():
             assert ((qb * s[i, j] - blk).abs() <= blk.abs() / 16 + s[i, j] * 2.0 ** -10).all()
     with pytest.raises(_lib.HgaError):
         ops.fp8_quantize_weight(w[0])
+
+
+def test_fp8_concat_lines_up_blocks():
+    import torch.nn as nn
+    from hierarchicalglobalattention_b200.fp8 import Fp8Linear, fp8_concat, fp8_weight_of
+    torch.manual_seed(0)
+    a, b, c = nn.Linear(200, 256, bias=False), nn.Linear(200, 128), nn.Linear(200, 30, bias=False)
+    w, s, bias = fp8_concat([a, b, c])
+    assert w.shape == (414, 200) and s.shape == (4, 2) and bias.shape == (414,)
+    assert torch.equal(bias[256:384], b.bias) and (bias[:256] == 0).all() and (bias[384:] == 0).all()
+    qa, sa = ops.fp8_quantize_weight(a.weight.detach())
+    assert torch.equal(w[:256].float(), qa.float()) and torch.equal(s[:2], sa)
+    assert fp8_concat([c, a]) is None                       # 30 features end inside a block
+    assert fp8_concat([a, nn.ReLU()]) is None
+    with pytest.raises(_lib.HgaError):
+        fp8_concat([a, nn.Linear(100, 128)])
+    m = Fp8Linear.from_linear(b)
+    got = fp8_weight_of(m)
+    assert torch.equal(got[0].float(), m.weight.float()) and torch.equal(got[2], b.bias)
+    assert fp8_weight_of(a) is None and set(m.state_dict()) == {"weight", "weight_scale_inv", "bias"}
+
+
+def test_low_bit_options_are_validated():
+    import types
+    import torch.nn as nn
+    import hierarchicalglobalattention_b200 as hga
+    with pytest.raises(ValueError, match="kv_bits"):
+        hga.HierarchicalGlobalAttentionRouted(d_model=64, nhead=4, kv_heads=2, kv_bits=8)
+    cfg = types.SimpleNamespace(num_attention_heads=4, num_key_value_heads=2, head_dim=64, hidden_size=64)
+    with pytest.raises(ValueError, match="kv_bits"):
+        hga.QwenRoutedAttention(nn.Identity(), cfg, kv_bits=2)
+    with pytest.raises(ValueError, match="Dual Chunk"):
+        hga.QwenRoutedAttention(nn.Identity(), cfg, kv_bits=4, dca_chunk=256)
+
+
+def test_fake_shapes_of_the_dispatcher_ops():
+    from hierarchicalglobalattention_b200 import torch_ops
+    m = dict(device="meta", dtype=torch.bfloat16)
+    x = torch.empty(3, 5, 300, **m)
+    q, s = torch.ops.hga.fp8_quantize(x)
+    assert q.shape == x.shape and q.dtype == torch.float8_e4m3fn and s.shape == (3, 5, 3) and s.dtype == torch.float32
+    w, ws = torch.empty(200, 300, device="meta", dtype=torch.float8_e4m3fn), torch.empty(2, 3, device="meta")
+    y = torch.ops.hga.fp8_linear(x, w, ws, None, None, None)
+    assert y.shape == (3, 5, 200) and y.dtype == torch.bfloat16
+    assert torch.ops.hga.fp8_linear(q, w, ws, None, s, torch.float32).dtype == torch.float32
+    k = torch.empty(2, 4, 100, 128, **m)
+    rk, rv = torch.ops.hga.kv4_pack(k, k)
+    assert rk.shape == (2, 4, 7, 1280) and rv.dtype == torch.uint8
+    assert torch.ops.hga.kv4_unpack(rk, rv, 100, torch.bfloat16)[0].shape == k.shape
+    p = _lib.make_params(batch=2, nhead=8, kv_heads=4, head_dim=128, chunk_size=64, group_size=16, topk_chunks=4,
+                         topk_groups=8, keep_first=1, keep_last=2, theta=1e4, dtype=torch.bfloat16)
+    pi, pf = torch_ops.params_lists(p)
+    qd = torch.empty(2, 8, 1, 128, **m)
+    i32 = dict(device="meta", dtype=torch.int32)
+    out = torch.ops.hga.attend_decode_kv4(pi, pf, qd, torch.empty(2, **i32), k, k, rk, rv, torch.empty(2, 8, 8, **i32),
+                                          torch.empty(2, 8, 8, **i32))
+    assert out.shape == qd.shape
