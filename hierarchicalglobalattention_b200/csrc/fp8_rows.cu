@@ -5,10 +5,11 @@
 // a fixed order (no atomics, no second launch).
 //   warp 0     TMA producer of the weight's (and, when x comes quantised, the tokens') 128-channel blocks
 //   warp 1     MMA issuer, TMEM owner: one group of four K = 32 steps per block into its own TMEM columns
-//   warps 2-5  FUSED: quantise the CTA's slice of x straight into the swizzled shared operand while the
-//              weight is on its way (each slice is small and comes from L2); then one feature a thread:
-//              sum[token] += D * (ws * xs[token]) per block
-// FUSED saves the quantisation's launch and its round trip through memory.
+//   warps 2-9  FUSED: quantise the CTA's slice of x straight into the swizzled shared operand while the
+//              weight is on its way (each slice is small and comes from L2)
+//   warps 2-5  then one feature a thread: sum[token] += D * (ws * xs[token]) per block
+// FUSED saves the quantisation's launch and its round trip through memory; past some 64 blocks a CTA its
+// repetition in every CTA costs more than that (16 x 8192 into 8192 features: 22.3 us against 14.2).
 #include <cooperative_groups.h>
 
 #include "fp8_common.cuh"
@@ -19,7 +20,7 @@ namespace tc {
 
 namespace cg = cooperative_groups;
 
-constexpr int kRowsThreads = 192;
+__host__ __device__ constexpr int rows_threads(bool fused) { return fused ? 320 : 192; }
 constexpr int kErrFp8Rows = 0x48;
 constexpr int kMaxSlice = 16;  // channel blocks per CTA
 
@@ -38,7 +39,7 @@ struct RowsArgs {
 };
 
 template <int TN, bool FUSED> struct RowsSmem {
-  static constexpr int kStages = TN == 64 ? 4 : 5;
+  static constexpr int kStages = FUSED || TN == 64 ? 4 : 5;  // two CTAs fit an SM
   static constexpr int kBufs = TN == 64 ? 4 : 8;               // TMEM buffers of TN columns
   static constexpr int kW = 128 * 128, kX = TN * 128;
   static constexpr int kStage = kW + (FUSED ? 0 : kX);
@@ -53,9 +54,10 @@ template <int TN, bool FUSED> struct RowsSmem {
 };
 
 template <typename TX, typename TO, int TN, bool FUSED>
-__global__ void __launch_bounds__(kRowsThreads)
+__global__ void __launch_bounds__(rows_threads(FUSED))
     fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const RowsArgs a) {
   using S = RowsSmem<TN, FUSED>;
+  constexpr int kRowsThreads = rows_threads(FUSED), kWork = kRowsThreads - 64;  // threads of warps 2 on
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   // every CTA of a cluster places its parts at the same offset (the distributed reads need that): the
   // dynamic base is the same in all of them
@@ -70,7 +72,7 @@ __global__ void __launch_bounds__(kRowsThreads)
   int* misc = reinterpret_cast<int*>(smem + S::kMisc);
   volatile int* abort_flag = misc;
   uint32_t* tmem_s = reinterpret_cast<uint32_t*>(misc + 1);
-  float* scale_s = reinterpret_cast<float*>(smem + S::kScale);
+  float* scale_s = reinterpret_cast<float*>(smem + S::kScale);  // token's scale x weight block's scale
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, n0 = blockIdx.y * 128, t0 = blockIdx.z * TN;
   const int kb0 = (int)((int64_t)a.kb * rank / a.splits), kb1 = (int)((int64_t)a.kb * (rank + 1) / a.splits);
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(kRowsThreads)
       mbar_init(d_full + i, 1);
       mbar_init(d_empty + i, 4);
     }
-    mbar_init(x_ready, 128);
+    mbar_init(x_ready, kWork);
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort_flag = 0;
@@ -140,59 +142,59 @@ __global__ void __launch_bounds__(kRowsThreads)
       mbar_drain(drain, 0);
     }
   } else {
-    const int e = tid - 64;  // 0..127
+    const int e = tid - 64;  // 0..kWork-1
     if constexpr (FUSED) {
-      // 16 lanes a block of 128 channels; the (block, row) pairs of the CTA's slice are dealt to the 8 half
-      // warps, four loads in flight each.  The operand's 128-byte swizzle: 16-byte piece p of row r sits at
+      // 16 lanes a block of 128 channels; the (block, row) pairs of the CTA's slice are dealt to the 16 half
+      // warps, two side by side each.  The operand's 128-byte swizzle: 16-byte piece p of row r sits at
       // p ^ (r & 7).  Rows past m are zeros with scale 0.
       const TX* x = static_cast<const TX*>(a.x);
+      const float* ws = a.ws + (int64_t)blockIdx.y * a.ws_stride + kb0;
       const int sub = e & 15, live = a.m - t0 < TN ? a.m - t0 : TN, pairs = nkb * live;
-      constexpr int R = 4;
-      for (int i = e; i < nkb * (TN - live) * 8; i += 128) {
+      constexpr int R = 2;
+      for (int i = e; i < nkb * (TN - live) * 8; i += kWork) {
         const int blk = i / ((TN - live) * 8), pc = i % ((TN - live) * 8);
         *reinterpret_cast<uint4*>(smem + S::kXs + blk * S::kX + live * 128 + pc * 16) = make_uint4(0u, 0u, 0u, 0u);
       }
-      for (int i = e; i < nkb * TN; i += 128) {
+      for (int i = e; i < nkb * TN; i += kWork) {
         if (i % TN >= live) scale_s[i] = 0.f;
       }
-      for (int base = (e >> 5) * 2; base < pairs; base += 8 * R) {
+      for (int base = (e >> 5) * 2; base < pairs; base += 16 * R) {
         Raw8<TX> f[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int pr = base + r * 8 + ((e >> 4) & 1);
+          const int pr = base + r * 16 + ((e >> 4) & 1);
           const int c0 = (kb0 + pr / live) * 128 + sub * 8;
           f[r] = pr < pairs ? raw_load<TX>(x + (int64_t)(t0 + pr % live) * a.x_stride + c0, a.x_vec, a.k - c0)
                             : raw_zero<TX>();
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          if (base + r * 8 >= pairs) break;  // warp-uniform
-          const int pr = base + r * 8 + ((e >> 4) & 1);
+          const int pr = base + r * 16 + ((e >> 4) & 1);
           uint2 v;
           const float s = fp8_block<TX>(f[r], v);
           if (pr < pairs) {
             const int blk = pr / live, row = pr % live;
             *reinterpret_cast<uint2*>(smem + S::kXs + blk * S::kX + row * 128 + (((sub >> 1) ^ (row & 7)) << 4) +
                                       (sub & 1) * 8) = v;
-            if (sub == 0) scale_s[blk * TN + row] = s;
+            if (sub == 0) scale_s[blk * TN + row] = s * ws[blk];
           }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     } else {
-      for (int i = e; i < nkb * TN; i += 128) {
+      for (int i = e; i < nkb * TN; i += kWork) {
         const int r = t0 + i % TN;
-        scale_s[i] = r < a.m ? a.xs[(int64_t)r * a.xs_stride + kb0 + i / TN] : 0.f;
+        scale_s[i] = r < a.m ? a.xs[(int64_t)r * a.xs_stride + kb0 + i / TN] *
+                                   a.ws[(int64_t)blockIdx.y * a.ws_stride + kb0 + i / TN]
+                             : 0.f;
       }
     }
     mbar_arrive(x_ready);
-    asm volatile("bar.sync 1, 128;" ::: "memory");  // the scales are in shared memory
+    asm volatile("bar.sync 1, %0;" ::"n"(kWork) : "memory");  // the scales are in shared memory
     const int quarter = warp & 3;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const float* ws = a.ws + (int64_t)blockIdx.y * a.ws_stride + kb0;
-    for (int it = 0; it < nkb; ++it) {
+    for (int it = 0; it < nkb && warp < 6; ++it) {
       const int buf = it % S::kBufs;
-      const float w = ws[it];
       if (!__all_sync(0xffffffffu, mbar_wait(d_full + buf, (it / S::kBufs) & 1, abort_flag, kErrFp8Rows + 4))) break;
       fence_after();
       uint32_t r[TN];
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kRowsThreads)
       __syncwarp();
       if (lane == 0) mbar_arrive(d_empty + buf);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[j] = fmaf(__uint_as_float(r[j]), scale_s[it * TN + j] * w, acc[j]);
+      for (int j = 0; j < TN; ++j) acc[j] = fmaf(__uint_as_float(r[j]), scale_s[it * TN + j], acc[j]);
     }
   }
 
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(kRowsThreads)
   TO* out = static_cast<TO*>(a.out);
   const TO* bias = static_cast<const TO*>(a.bias);
   if (a.splits == 1) {
-    if (warp >= 2 && n0 + feat < a.n) {
+    if (warp >= 2 && warp < 6 && n0 + feat < a.n) {
       const float add = bias ? Num<TO>::to_f(bias[n0 + feat]) : 0.f;
 #pragma unroll
       for (int j = 0; j < TN; ++j)
@@ -228,21 +230,43 @@ __global__ void __launch_bounds__(kRowsThreads)
     // the ring is free: the last block's MMAs (which read it) have completed and no load is outstanding
     float* part = reinterpret_cast<float*>(smem);  // [TN][128]
     __syncthreads();
-    if (warp >= 2) {
+    if (warp >= 2 && warp < 6) {
 #pragma unroll
       for (int j = 0; j < TN; ++j) part[j * 128 + feat] = acc[j];
     }
     cg::cluster_group cl = cg::this_cluster();
     __syncwarp();
     cl.sync();
+    // this CTA's share of the tile, four features of a token at a time, the CTAs' sums in rank order
     const int lo = TN * rank / a.splits, hi = TN * (rank + 1) / a.splits;
-    for (int i = lo * 128 + tid; i < hi * 128; i += kRowsThreads) {
-      const int j = i >> 7, f = i & 127;
-      if (t0 + j < a.m && n0 + f < a.n) {
-        float s = 0.f;
-        for (int p = 0; p < a.splits; ++p) s += *cl.map_shared_rank(part + i, p);
-        if (bias) s += Num<TO>::to_f(bias[n0 + f]);
-        out[(int64_t)(t0 + j) * a.out_stride + n0 + f] = Num<TO>::from_f(s);
+    for (int i = lo * 32 + tid; i < hi * 32; i += kRowsThreads) {
+      const int j = i >> 5, f = (i & 31) * 4;
+      if (t0 + j >= a.m || n0 + f >= a.n) continue;
+      float4 v[8];
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        if (p < a.splits) v[p] = *cl.map_shared_rank(reinterpret_cast<float4*>(part) + i, p);
+      float o[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+      for (int p = 1; p < 8; ++p)
+        if (p < a.splits) {
+          o[0] += v[p].x;
+          o[1] += v[p].y;
+          o[2] += v[p].z;
+          o[3] += v[p].w;
+        }
+      TO* dst = out + (int64_t)(t0 + j) * a.out_stride + n0 + f;
+      TO y[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        y[c] = Num<TO>::from_f(o[c] + (bias && n0 + f + c < a.n ? Num<TO>::to_f(bias[n0 + f + c]) : 0.f));
+      if (n0 + f + 4 <= a.n && ((uintptr_t)dst & (4 * sizeof(TO) - 1)) == 0) {
+        if constexpr (sizeof(TO) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (n0 + f + c < a.n) dst[c] = y[c];
       }
     }
     cl.sync();  // no CTA leaves while another still reads its sums
@@ -294,7 +318,7 @@ static cudaError_t rows_t(const Fp8Linear& a, const void* q, int64_t q_stride, c
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(r.splits, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + TN - 1) / TN));
-  cfg.blockDim = dim3(kRowsThreads);
+  cfg.blockDim = dim3(rows_threads(FUSED));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -311,8 +335,10 @@ static cudaError_t rows_m(const Fp8Linear& a, const void* q, int64_t q_stride, c
                           const void* w, int64_t w_stride, cudaStream_t st) {
   const int tn = rows_tn(a.m);
   if (tn == 16) return rows_t<TX, TO, 16, FUSED>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
-  if (tn == 32) return rows_t<TX, TO, 32, FUSED>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
-  if constexpr (!FUSED) return rows_t<TX, TO, 64, false>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  if constexpr (!FUSED) {
+    if (tn == 32) return rows_t<TX, TO, 32, false>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+    return rows_t<TX, TO, 64, false>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  }
   return cudaErrorInvalidValue;
 }
 
@@ -335,10 +361,21 @@ static bool rows_fit(const Fp8Linear& a) {
   return kb <= 8 * tc::kMaxSlice && (a.n + 127) / 128 <= 65535;
 }
 
-// Rows for which streaming the weight is better than 128-row tiles.
-bool fp8_rows_better(const Fp8Linear& a) { return a.m <= 256 && rows_fit(a); }
+// Where the weight is read by CTAs that are all resident at once (two an SM, four along the channels) this
+// kernel is ahead of the 128-row tiles, which have fewer CTAs and walk all channels in each: 128 rows of 4096
+// channels into 2048 features 13.4 against 19.1 us, 64 of 2048 into 5120 11.7 against 12.9; past that
+// behind: 128 of 2048 into 5120 14.9 against 13.4.
+bool fp8_rows_better(const Fp8Linear& a) {
+  const int tn = tc::rows_tn(a.m);
+  return rows_fit(a) && (a.m <= 64 || (a.n + 127) / 128 * ((a.m + tn - 1) / tn) <= 64);
+}
 
-bool fp8_rows_fused(const Fp8Linear& a) { return a.x_dtype != HGA_DTYPE_E4M3 && a.m <= 32 && rows_fit(a); }
+// Quantising inside pays as long as a CTA has no more than about 64 (row, block) pairs of its own.
+bool fp8_rows_fused(const Fp8Linear& a) {
+  if (a.x_dtype == HGA_DTYPE_E4M3 || a.m > 16 || !rows_fit(a)) return false;
+  const int64_t kb = (a.k + 127) / 128, splits = tc::rows_splits(a.m, a.n, kb, 16);
+  return a.m * ((kb + splits - 1) / splits) <= 64;
+}
 
 cudaError_t launch_fp8_rows(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
                             const void* w, int64_t w_stride, cudaStream_t st) {

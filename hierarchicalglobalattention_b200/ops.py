@@ -382,8 +382,6 @@ FP8_BLOCK = 128
 _FP8_X = {**_lib.DTYPE_CODE, torch.float8_e4m3fn: _lib.E4M3_CODE}
 
 
-# rows up to which hga_fp8_linear needs no workspace when its operands are 16-byte aligned
-_FP8_NO_WORKSPACE = 32
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -479,11 +477,8 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
         raise _lib.HgaError("fp8_linear: out must be a contiguous [..., N] tensor of the result's type")
     h = lib()
     xp, wp, xst, wst = r.data_ptr(), w.data_ptr(), max(r.stride(0), K), max(w.stride(0), K)
-    need, ws = 0, None
-    if M > _FP8_NO_WORKSPACE or code == _lib.E4M3_CODE or (wp | wst) & 15 or K > 16384:
-        need = h.hga_fp8_linear_workspace(M, N, K, code, xp, xst, wp, wst)
-        if need:
-            ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    need = h.hga_fp8_linear_workspace(M, N, K, code, xp, xst, wp, wst)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     rc = h.hga_fp8_linear(M, N, K, code, xp, xst, None if xs is None else xs.data_ptr(), wp, wst, w_scale.data_ptr(),
                           max(w_scale.stride(0), KB), None if bias is None else bias.data_ptr(), ocode, out.data_ptr(),
                           N, None if ws is None else ws.data_ptr(), need, stream_ptr(dev))
