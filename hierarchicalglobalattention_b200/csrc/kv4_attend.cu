@@ -13,9 +13,10 @@
 //   o     = sum_keys    w (n - 8) + p mid_b,                         w = bf16(p scale_b)
 // so keys enter the scores unrounded, and a weight's product with the block's scale is rounded to bf16 once
 // (as the weights of any 16-bit attention are; fp16 results carry three more bits, so there w is two bf16
-// terms, and fp16 itself would lose small scales to its range).  The mid terms are fp32 sums beside the products.  Leaving
-// the 128 or 1024 in the products and taking its sum off afterwards saves the subtractions but costs the
-// scores up to 1 % in fp16: the instruction truncates its sums relative to their largest term.
+// terms, and fp16 itself would lose small scales to its range).  The mid terms are fp32 sums beside the
+// products.  bf16 scores leave the 128 in the products and take 128 sum q off instead; with fp16's 1024 that cost
+// up to 1 % of a score (the instruction truncates its sums relative to their largest term), and in the
+// output, whose sum runs over all keys, a bf16 ulp.
 //
 // Units are dealt to the 8 warps of the `splits` CTAs of a cluster (windows and the active chunk first,
 // then the union); every warp keeps its own online softmax and copies its next units with cp.async (plain
@@ -24,6 +25,7 @@
 // Bound by HBM when many sequences decode, by latency for one.
 #include <cooperative_groups.h>
 
+#include "fp32x2.cuh"
 #include "kv4_common.cuh"
 
 namespace hga {
@@ -89,6 +91,12 @@ __device__ __forceinline__ uint32_t codes(uint32_t word, int i) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// whether the scale or the minimum of a word is not finite
+template <typename H>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  return ((w >> 16) & H::kInf) == H::kInf || (w & H::kInf) == H::kInf;
+}
+
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (Half2<T>::kInf == 0x7f80u)
@@ -136,7 +144,7 @@ __device__ __forceinline__ uint4 load16(const void* p) {
 template <int DH, int NT> struct Layout {
   static constexpr int kOut = DH * 8 * NT * 4;                       // one partial O^T, fp32
   static constexpr int kRing = kWarps * Buf<DH>::kWarp;
-  static constexpr int kPart = (kWarps + 1) * kOut + (kWarps + 1) * 2 * 8 * NT * 4;
+  static constexpr int kPart = kWarps * kOut + 8 * NT * (DH + 4) * 4 + (kWarps + 1) * 2 * 8 * NT * 4;
   static constexpr int kQ = kRing > kPart ? kRing : kPart;           // [NT][DH/16][32] uint2: Q as B fragments
   static constexpr int kScratch = kQ + NT * (DH / 16) * 32 * 8;      // [warps][16][8 NT] fp32 weights (rare path)
   static constexpr int kMisc = kScratch + kWarps * 16 * 8 * NT * 4;
@@ -153,6 +161,10 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   using H = Half2<T>;
   using LY = Layout<DH, NT>;
   constexpr int KS = DH / 16, NB = DH / 32, COLS = 8 * NT;
+  // what the keys' codes have in the products besides themselves: 8 off (n - 8), or 128 on (bf16 keeps it:
+  // 128 sum q is taken off in fp32 with an error of 1e-5 of a score)
+  constexpr bool FP16 = H::kInf != 0x7f80u;
+  constexpr float kOffK = FP16 ? 8.f : -128.f;
   constexpr bool SPLIT = H::kInf != 0x7f80u;  // fp16: the weights of the record as two bf16 terms
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -166,6 +178,18 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   int* misc = reinterpret_cast<int*>(smem + LY::kMisc);
 
   cg::cluster_group cl = cg::this_cluster();
+  // the first entries of the heads' lists (one or two a thread: all of them for 64 groups and 8 heads), asked
+  // for before anything waits for the sequence's position
+  const int N = hr * Kg, hsize = 1 << a.hash_bits;
+  const size_t list0 = ((size_t)b * p.nhead + h0) * Kg;
+  constexpr int kEarly = 2;
+  int e_gid[kEarly], e_t0[kEarly];
+#pragma unroll
+  for (int j = 0; j < kEarly; ++j) {
+    const int i = tid + j * kWarps * 32;
+    e_gid[j] = ncols > 0 && i < N ? a.open_gid[list0 + i] : -1;
+    e_t0[j] = ncols > 0 && i < N ? a.open_t0[list0 + i] : -1;
+  }
   if (ncols <= 0) return;  // the whole cluster: a smaller last head block has fewer tiles
   const int pos = a.seq_pos[b];
   const int n_closed = pos / C, c0 = pos % C;
@@ -237,7 +261,6 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   }
 
   // ---- union of the heads' opened groups --------------------------------------------------------
-  const int N = hr * Kg, hsize = 1 << a.hash_bits;
   int* keys = reinterpret_cast<int*>(smem + LY::kTables);  // [hsize] group, -1 empty
   int* own = keys + hsize;                                 // [hsize] first entry that names it
   int* rnk = own + hsize;                                  // [hsize] its place in the union
@@ -251,9 +274,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   }
   for (int i = tid; i < N * hr; i += kWarps * 32) ut0[i] = kNever;
   __syncthreads();
-  const size_t list0 = ((size_t)b * p.nhead + h0) * Kg;
-  for (int i = tid; i < N; i += kWarps * 32) {
-    const int gid = a.open_gid[list0 + i], t0 = a.open_t0[list0 + i];
+  auto insert = [&](int i, int gid, int t0) {
     int s = -1;
     if (gid >= 0 && t0 >= 0 && t0 <= t_last) {
       if ((int64_t)(gid + 1) * U > a.unit_cap) {
@@ -269,7 +290,11 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
       }
     }
     slot[i] = s;
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < kEarly; ++j)
+    if (tid + j * kWarps * 32 < N) insert(tid + j * kWarps * 32, e_gid[j], e_t0[j]);
+  for (int i = tid + kEarly * kWarps * 32; i < N; i += kWarps * 32) insert(i, a.open_gid[list0 + i], a.open_t0[list0 + i]);
   __syncthreads();
   // places in the order of the first entries (the same in every run, whatever slot the hash gave)
   int n_open = 0;
@@ -294,7 +319,12 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
     n_open += total;
     __syncthreads();
   }
-  for (int i = tid; i < N; i += kWarps * 32)
+#pragma unroll
+  for (int j = 0; j < kEarly; ++j) {
+    const int i = tid + j * kWarps * 32;
+    if (i < N && slot[i] >= 0) ut0[rnk[slot[i]] * hr + i / Kg] = (uint8_t)e_t0[j];
+  }
+  for (int i = tid + kEarly * kWarps * 32; i < N; i += kWarps * 32)
     if (slot[i] >= 0) ut0[rnk[slot[i]] * hr + i / Kg] = (uint8_t)a.open_t0[list0 + i];
   __syncthreads();
 
@@ -476,7 +506,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   constexpr int QUADS = DH / 64;
   // a lane copies the code words that it will read itself, and one 16-byte piece of the (scale, min) pairs
   auto issue_rec = [&](int u, int st) {
-    const int64_t unit = (int64_t)ugid[u / U] * U + u % U;
+    const int64_t unit = U == 1 ? (int64_t)ugid[u] : (int64_t)ugid[u / U] * U + u % U;
     const uint8_t* ks = a.rec_k + rec_base + unit * kv4_unit_bytes(DH);
     const uint8_t* vs = a.rec_v + rec_base + unit * kv4_unit_bytes(DH);
     unsigned char* d = buf + st * Buf<DH>::kUnit;
@@ -553,7 +583,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
         for (int k = 0; k < 2; ++k) {
           uint32_t f[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = codes<H>(word[hb2 * 2 + k], e);
+          for (int e = 0; e < 4; ++e) f[e] = SPLIT ? codes<H>(word[hb2 * 2 + k], e) : (word[hb2 * 2 + k] >> (4 * e) & 0x000f000fu) | H::kMagic;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const uint2 v = qf[(nt * KS + blk * 2 + k) * 32 + lane];
@@ -562,23 +592,32 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float sc = H::lo(km[r][blk]), mid = fmaf(8.f, sc, H::hi(km[r][blk]));
+          const float sc = H::lo(km[r][blk]), mid = fmaf(kOffK, sc, H::hi(km[r][blk]));
+          const uint64_t sc2 = f32x2(sc, sc), mid2 = f32x2(mid, mid);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              s[nt][2 * r + e] = fmaf(sc, acc[nt][2 * r + e], fmaf(mid, qsum[blk][nt][e], s[nt][2 * r + e]));
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint64_t q2 = f32x2(qsum[blk][nt][0], qsum[blk][nt][1]);
+            f32x2_get(f32x2_fma(sc2, f32x2(acc[nt][2 * r], acc[nt][2 * r + 1]),
+                                f32x2_fma(mid2, q2, f32x2(s[nt][2 * r], s[nt][2 * r + 1]))),
+                      s[nt][2 * r], s[nt][2 * r + 1]);
+          }
         }
       }
     }
     unsigned vis[NT];
-    const uint8_t* t0 = ut0 + (u / U) * hr;
+    const uint8_t* t0 = ut0 + (U == 1 ? u : u / U) * hr;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
       vis[nt] = (col_t[nt][0] >= t0[col_h[nt][0]] ? 5u : 0u) | (col_t[nt][1] >= t0[col_h[nt][1]] ? 10u : 0u);
     soften(s, vis);
-    // values
+    // values; odd: a block of the unit reads back as NaN, which columns that do not see the unit must not meet
     const unsigned char* dv = d + 10 * DH;
+    bool odd = false;
+    if (lane < NB * 4) {
+      const uint4 m4 = *reinterpret_cast<const uint4*>(dv + 8 * DH + lane * 16);
+      odd = not_finite<H>(m4.x) | not_finite<H>(m4.y) | not_finite<H>(m4.z) | not_finite<H>(m4.w);
+    }
+    odd = __any_sync(0xffffffffu, odd);
 #pragma unroll
     for (int quad = 0; quad < QUADS; ++quad) {
       const uint4 w4 = *reinterpret_cast<const uint4*>(dv + (quad * 32 + lane) * 16);
@@ -591,15 +630,24 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
         for (int r = 0; r < 2; ++r) {
           const uint32_t vm = *reinterpret_cast<const uint32_t*>(dv + 8 * DH + ((g + 8 * r) * NB + blk) * 4);
           const float sc = H::lo(vm), mid = fmaf(8.f, sc, H::hi(vm));
+          const uint64_t sc2 = f32x2(sc, sc), mid2 = f32x2(mid, mid);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            // an unseen key's scale and minimum do not count, whatever they hold
-            const bool v0 = vis[nt] & 1u, v1 = vis[nt] & 2u;
-            const float w0 = v0 ? s[nt][2 * r] * sc : 0.f, w1 = v1 ? s[nt][2 * r + 1] * sc : 0.f;
+            const uint64_t p2 = f32x2(s[nt][2 * r], s[nt][2 * r + 1]);
+            float w0, w1, d0, d1;
+            f32x2_get(f32x2_mul(p2, sc2), w0, w1);
+            f32x2_get(f32x2_fma(p2, mid2, f32x2(corr[blk][nt][0], corr[blk][nt][1])), d0, d1);
+            if (odd) {  // an unseen key's scale and minimum do not count, whatever they hold
+              const bool v0 = vis[nt] & 1u, v1 = vis[nt] & 2u;
+              w0 = v0 ? w0 : 0.f;
+              w1 = v1 ? w1 : 0.f;
+              d0 = v0 ? d0 : corr[blk][nt][0];
+              d1 = v1 ? d1 : corr[blk][nt][1];
+            }
+            corr[blk][nt][0] = d0;
+            corr[blk][nt][1] = d1;
             const uint32_t w = BF::pack(w0, w1);
             if constexpr (SPLIT) wl[nt][r] = transpose8(BF::pack(w0 - BF::lo(w), w1 - BF::hi(w)));
-            corr[blk][nt][0] = v0 ? fmaf(s[nt][2 * r], mid, corr[blk][nt][0]) : corr[blk][nt][0];
-            corr[blk][nt][1] = v1 ? fmaf(s[nt][2 * r + 1], mid, corr[blk][nt][1]) : corr[blk][nt][1];
             wb[nt][r] = transpose8(w);
           }
         }
@@ -638,8 +686,8 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
       }
     }
   __syncthreads();  // the copy buffers become the partial results
-  float* part = reinterpret_cast<float*>(smem);                 // [warps + 1][DH][COLS]
-  float* pm = part + (kWarps + 1) * DH * COLS;                  // [warps + 1][COLS] maxima
+  float* part = reinterpret_cast<float*>(smem);                 // [warps][DH][COLS], then the CTA's [COLS][DH + 4]
+  float* pm = part + kWarps * DH * COLS + COLS * (DH + 4);       // [warps + 1][COLS] maxima
   float* pl = pm + (kWarps + 1) * COLS;                         // [warps + 1][COLS] sums
 #pragma unroll
   for (int i = 0; i < KS; ++i)
@@ -671,6 +719,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
     pl[kWarps * COLS + tid] = sum;
   }
   __syncthreads();
+  constexpr int MS = DH + 4;  // the CTA's result, [COLS][MS]: channels next to one another
   float* mine = part + kWarps * DH * COLS;
   for (int i = tid; i < DH * COLS; i += kWarps * 32) {
     float s = 0.f;
@@ -679,27 +728,34 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
       const float f = pm[w * COLS + i % COLS];
       s += f == 0.f ? 0.f : f * part[w * DH * COLS + i];
     }
-    mine[i] = s;
+    mine[(i % COLS) * MS + i / COLS] = s;
   }
   if (a.splits > 1) cl.sync(); else __syncthreads();
-  const int lo = DH * rank / a.splits, hi = DH * (rank + 1) / a.splits;
-  for (int i = tid; i < (hi - lo) * COLS; i += kWarps * 32) {
-    const int col = i / (hi - lo), ch = lo + i % (hi - lo);
-    if (col >= ncols) break;
-    float mx = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int r = 0; r < a.splits; ++r) {
+  // this CTA's share of the channels, the CTAs' results in rank order (all of an element's reads in flight
+  // together: one after the other they took as long as the attention of a short context)
+  const int lo = DH * rank / a.splits, width = DH * (rank + 1) / a.splits - lo;
+  for (int i = tid; i < width * ncols; i += kWarps * 32) {
+    const int col = i / width, ch = lo + i % width;
+    float mr[8], lr[8], vr[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (r >= a.splits) break;
       const float* rm = a.splits > 1 ? cl.map_shared_rank(pm, r) : pm;
-      mx = fmaxf(mx, rm[kWarps * COLS + col]);
+      mr[r] = rm[kWarps * COLS + col];
+      lr[r] = rm[(2 * kWarps + 1) * COLS + col];  // pl follows pm
+      vr[r] = (a.splits > 1 ? cl.map_shared_rank(mine, r) : mine)[col * MS + ch];
     }
-    for (int r = 0; r < a.splits; ++r) {
-      const float* rm = a.splits > 1 ? cl.map_shared_rank(pm, r) : pm;
-      const float* rl = a.splits > 1 ? cl.map_shared_rank(pl, r) : pl;
-      const float* ro = a.splits > 1 ? cl.map_shared_rank(mine, r) : mine;
-      const float mr = rm[kWarps * COLS + col];
-      const float lr = rl[kWarps * COLS + col], f = mr == -INFINITY ? lr : ex2(mr - mx);
+    float mx = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < a.splits) mx = fmaxf(mx, mr[r]);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (r >= a.splits) break;
+      const float f = mr[r] == -INFINITY ? lr[r] : ex2(mr[r] - mx);
       if (f == 0.f) continue;
-      sum += f * lr;
-      acc += f * ro[ch * COLS + col];
+      sum += f * lr[r];
+      acc += f * vr[r];
     }
     const int x = x0 + col;
     out[(((size_t)b * p.nhead + h0 + x % hr) * L + x / hr) * DH + ch] = Num<T>::from_f(sum == 0.f ? 0.f : acc / sum);
