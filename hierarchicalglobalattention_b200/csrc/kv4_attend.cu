@@ -43,7 +43,10 @@ constexpr int kNever = 255;         // t0 of a (unit, head) that does not see th
 template <int DH> struct Buf {
   static constexpr int kUnit = 20 * DH;                                          // K and V of a record unit
   static constexpr int kHot = 2 * 16 * DH * 2;                                   // K and V rows of a slot unit
-  static constexpr int kWarp = kStages * kUnit > kHot ? kStages * kUnit : kHot;
+  // the last stage lies behind the slot unit's rows: the first record unit is on its way while those are attended
+  static constexpr int kRing = kHot - (kStages - 1) * kUnit;                     // offset of stage 0
+  static constexpr int kWarp = kRing + kStages * kUnit;
+  static_assert(kRing >= 0 && kRing % 16 == 0 && kWarp - kUnit >= kHot, "stage kStages - 1 is clear of the slot rows");
 };
 
 struct Args {
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   int* slot = rnk + hsize;                                 // [N] hash slot of an entry, -1 skipped
   int* ugid = slot + N;                                    // [N] the union's groups
   uint8_t* ut0 = reinterpret_cast<uint8_t*>(ugid + N);     // [N][hr] first row that sees it
-  int* wcnt = misc + 4;                                    // [warps]
+  int* wcnt = misc;                                        // [2][warps]
   for (int i = tid; i < hsize; i += kWarps * 32) {
     keys[i] = -1;
     own[i] = 0x7fffffff;
@@ -298,25 +301,32 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   __syncthreads();
   // places in the order of the first entries (the same in every run, whatever slot the hash gave)
   int n_open = 0;
-  for (int base = 0; base < N; base += kWarps * 32) {
-    const int i = base + tid;
-    const bool first = i < N && slot[i] >= 0 && own[slot[i]] == i;
-    const unsigned bal = __ballot_sync(0xffffffffu, first);
-    if (lane == 0) wcnt[warp] = __popc(bal);
-    __syncthreads();
-    int before = n_open, total = 0;
+  for (int base = 0; base < N; base += 2 * kWarps * 32) {  // two entries a thread and round
+    bool first[2];
+    unsigned bal[2];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int j = 0; j < 2; ++j) {
+      const int i = base + j * kWarps * 32 + tid;
+      first[j] = i < N && slot[i] >= 0 && own[slot[i]] == i;
+      bal[j] = __ballot_sync(0xffffffffu, first[j]);
+      if (lane == 0) wcnt[j * kWarps + warp] = __popc(bal[j]);
+    }
+    __syncthreads();
+    int before[2] = {n_open, n_open};
+#pragma unroll
+    for (int w = 0; w < 2 * kWarps; ++w) {
       const int x = wcnt[w];
-      if (w < warp) before += x;
-      total += x;
+      if (w < warp) before[0] += x;
+      if (w < kWarps + warp) before[1] += x;
+      n_open += x;
     }
-    if (first) {
-      const int r = before + __popc(bal & ((1u << lane) - 1u));
-      rnk[slot[i]] = r;
-      ugid[r] = keys[slot[i]];
-    }
-    n_open += total;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (first[j]) {
+        const int sl = slot[base + j * kWarps * 32 + tid], r = before[j] + __popc(bal[j] & ((1u << lane) - 1u));
+        rnk[sl] = r;
+        ugid[r] = keys[sl];
+      }
     __syncthreads();
   }
 #pragma unroll
@@ -411,9 +421,50 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
       }
   };
 
+  // ---- copies of opened groups ---------------------------------------------------------------------------------
+  // the warps go on where the slot units' deal ended, so that one extra slot unit is paid back here
+  const int n_units = n_open * U;
+  const int start = (me + stride - n_hot % stride) % stride;
+  const size_t rec_base = (size_t)bk * a.unit_cap * kv4_unit_bytes(DH);
+  constexpr int QUADS = DH / 64;
+  // a lane copies the code words that it will read itself, and one 16-byte piece of the (scale, min) pairs
+  auto issue_rec = [&](int u, int st) {
+    const int64_t unit = U == 1 ? (int64_t)ugid[u] : (int64_t)ugid[u / U] * U + u % U;
+    const uint8_t* ks = a.rec_k + rec_base + unit * kv4_unit_bytes(DH);
+    const uint8_t* vs = a.rec_v + rec_base + unit * kv4_unit_bytes(DH);
+    unsigned char* d = buf + Buf<DH>::kRing + st * Buf<DH>::kUnit;
+    constexpr int MP = DH / 8;  // 16-byte pieces of one operand's pairs
+    const uint8_t* ms = lane < MP ? ks + 8 * DH + lane * 16 : vs + 8 * DH + (lane - MP) * 16;
+    unsigned char* md = lane < MP ? d + 8 * DH + lane * 16 : d + 18 * DH + (lane - MP) * 16;
+    if (!a.direct) {
+#pragma unroll
+      for (int j = 0; j < QUADS; ++j) {
+        copy16(d + (j * 32 + lane) * 16, ks + (j * 32 + lane) * 16, true);
+        copy16(d + 10 * DH + (j * 32 + lane) * 16, vs + (j * 32 + lane) * 16, true);
+      }
+      if (lane < 2 * MP) copy16(md, ms, true);
+    } else {
+      uint4 x[2 * QUADS + 1];
+#pragma unroll
+      for (int j = 0; j < QUADS; ++j) {
+        x[2 * j] = load16(ks + (j * 32 + lane) * 16);
+        x[2 * j + 1] = load16(vs + (j * 32 + lane) * 16);
+      }
+      if (lane < 2 * MP) x[2 * QUADS] = load16(ms);
+#pragma unroll
+      for (int j = 0; j < QUADS; ++j) {
+        *reinterpret_cast<uint4*>(d + (j * 32 + lane) * 16) = x[2 * j];
+        *reinterpret_cast<uint4*>(d + 10 * DH + (j * 32 + lane) * 16) = x[2 * j + 1];
+      }
+      if (lane < 2 * MP) *reinterpret_cast<uint4*>(md) = x[2 * QUADS];
+    }
+  };
+  if (start < n_units) issue_rec(start, kStages - 1);
+  copy_commit();
+
   // ---- windows and the active chunk -----------------------------------------------------------------
   for (int i = me; i < n_hot; i += stride) {
-    copy_wait<0>();
+    if (i == me) copy_wait<1>(); else copy_wait<0>();  // the first was issued before the record's first unit
     __syncwarp();
     int rows, act;
     hot_unit(i, rows, act);
@@ -499,53 +550,16 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   }
 
   // ---- opened groups ---------------------------------------------------------------------------------
-  // the warps go on where the slot units' deal ended, so that one extra slot unit is paid back here
-  const int n_units = n_open * U;
-  const int start = (me + stride - n_hot % stride) % stride;
-  const size_t rec_base = (size_t)bk * a.unit_cap * kv4_unit_bytes(DH);
-  constexpr int QUADS = DH / 64;
-  // a lane copies the code words that it will read itself, and one 16-byte piece of the (scale, min) pairs
-  auto issue_rec = [&](int u, int st) {
-    const int64_t unit = U == 1 ? (int64_t)ugid[u] : (int64_t)ugid[u / U] * U + u % U;
-    const uint8_t* ks = a.rec_k + rec_base + unit * kv4_unit_bytes(DH);
-    const uint8_t* vs = a.rec_v + rec_base + unit * kv4_unit_bytes(DH);
-    unsigned char* d = buf + st * Buf<DH>::kUnit;
-    constexpr int MP = DH / 8;  // 16-byte pieces of one operand's pairs
-    const uint8_t* ms = lane < MP ? ks + 8 * DH + lane * 16 : vs + 8 * DH + (lane - MP) * 16;
-    unsigned char* md = lane < MP ? d + 8 * DH + lane * 16 : d + 18 * DH + (lane - MP) * 16;
-    if (!a.direct) {
 #pragma unroll
-      for (int j = 0; j < QUADS; ++j) {
-        copy16(d + (j * 32 + lane) * 16, ks + (j * 32 + lane) * 16, true);
-        copy16(d + 10 * DH + (j * 32 + lane) * 16, vs + (j * 32 + lane) * 16, true);
-      }
-      if (lane < 2 * MP) copy16(md, ms, true);
-    } else {
-      uint4 x[2 * QUADS + 1];
-#pragma unroll
-      for (int j = 0; j < QUADS; ++j) {
-        x[2 * j] = load16(ks + (j * 32 + lane) * 16);
-        x[2 * j + 1] = load16(vs + (j * 32 + lane) * 16);
-      }
-      if (lane < 2 * MP) x[2 * QUADS] = load16(ms);
-#pragma unroll
-      for (int j = 0; j < QUADS; ++j) {
-        *reinterpret_cast<uint4*>(d + (j * 32 + lane) * 16) = x[2 * j];
-        *reinterpret_cast<uint4*>(d + 10 * DH + (j * 32 + lane) * 16) = x[2 * j + 1];
-      }
-      if (lane < 2 * MP) *reinterpret_cast<uint4*>(md) = x[2 * QUADS];
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (start + i * stride < n_units) issue_rec(start + i * stride, i);
+  for (int i = 1; i < kStages - 1; ++i) {
+    if (start + i * stride < n_units) issue_rec(start + i * stride, i - 1);
     copy_commit();
   }
-  int st = 0;
+  int st = kStages - 1;
   for (int u = start; u < n_units; u += stride) {
     copy_wait<kStages - 2>();
     __syncwarp();
-    const unsigned char* d = buf + st * Buf<DH>::kUnit;
+    const unsigned char* d = buf + Buf<DH>::kRing + st * Buf<DH>::kUnit;
     {
       const int un = u + (kStages - 1) * stride;
       if (un < n_units) issue_rec(un, (st + kStages - 1) % kStages);
