@@ -6,6 +6,7 @@ there is no CPU path.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -384,6 +385,9 @@ _FP8_X = {**_lib.DTYPE_CODE, torch.float8_e4m3fn: _lib.E4M3_CODE}
 
 
 
+_FP8_FEW_ROWS = 16
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x [..., K] as [M, K] rows with unit stride in the last dimension (a view where one exists)."""
     if x.dim() != 2:
@@ -404,8 +408,8 @@ def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     K = shape[-1]
     r = x if len(shape) == 2 and x.is_contiguous() else _rows(x)
     dev = x.device
-    q = torch.empty(shape, device=dev, dtype=torch.float8_e4m3fn)
-    scale = torch.empty((*shape[:-1], -(-K // FP8_BLOCK)), device=dev, dtype=torch.float32)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    scale = x.new_empty((*shape[:-1], -(-K // FP8_BLOCK)), dtype=torch.float32)
     rc = lib().hga_fp8_quantize(r.shape[0], K, code, r.data_ptr(), max(r.stride(0), K), q.data_ptr(), K,
                                 scale.data_ptr(), stream_ptr(dev))
     if rc:
@@ -438,11 +442,13 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     128 channels on the way in; e4m3 rows come with ``x_scale`` [..., ceil(K / 128)], as fp8_quantize
     returns them.  The result [..., N] has ``out_dtype``: x's type, or bf16 for 8-bit x.  ``bias`` [N] has
     the result's type."""
-    dev = x.device
-    for t in (x, w, w_scale, bias, x_scale, out):
-        if t is not None and (not t.is_cuda or t.device != dev):
-            _require_cuda(t)
+    dev, idx = x.device, x.get_device()
+    for t in (w, w_scale, bias, x_scale, out):
+        if t is not None and t.get_device() != idx:
+            _require_cuda(x, t)
             raise _lib.HgaError("fp8_linear: tensors on different devices")
+    if idx < 0:
+        _require_cuda(x)
     code = _FP8_X.get(x.dtype)
     if code is None:
         raise _lib.HgaError(f"fp8_linear: x must be fp32, bf16, fp16 or e4m3; got {x.dtype}")
@@ -472,16 +478,21 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     r = x if len(shape) == 2 and x.is_contiguous() else _rows(x)
     M = r.shape[0]
     if out is None:
-        out = torch.empty((*shape[:-1], N), device=dev, dtype=out_dtype)
+        out = x.new_empty((*shape[:-1], N), dtype=out_dtype)
     elif out.dtype != out_dtype or out.shape != (*shape[:-1], N) or not out.is_contiguous():
         raise _lib.HgaError("fp8_linear: out must be a contiguous [..., N] tensor of the result's type")
     h = lib()
-    xp, wp, xst, wst = r.data_ptr(), w.data_ptr(), max(r.stride(0), K), max(w.stride(0), K)
+    xp, wp, xst, wst = r.data_ptr(), w.data_ptr(), r.stride(0), w.stride(0)
+    xst, wst, sst = xst if xst > K else K, wst if wst > K else K, w_scale.stride(0)
+    call = (M, N, K, code, xp, xst, None if xs is None else xs.data_ptr(), wp, wst, w_scale.data_ptr(),
+            sst if sst > KB else KB, None if bias is None else bias.data_ptr(), ocode, out.data_ptr(), N)
+    stream = stream_ptr(dev)
+    # few rows mostly need no workspace: asked for only when the call says so
+    if M <= _FP8_FEW_ROWS and h.hga_fp8_linear(*call, None, 0, stream) == 0:
+        return out
     need = h.hga_fp8_linear_workspace(M, N, K, code, xp, xst, wp, wst)
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-    rc = h.hga_fp8_linear(M, N, K, code, xp, xst, None if xs is None else xs.data_ptr(), wp, wst, w_scale.data_ptr(),
-                          max(w_scale.stride(0), KB), None if bias is None else bias.data_ptr(), ocode, out.data_ptr(),
-                          N, None if ws is None else ws.data_ptr(), need, stream_ptr(dev))
+    rc = h.hga_fp8_linear(*call, None if ws is None else ws.data_ptr(), need, stream)
     if rc:
         check(rc, "hga_fp8_linear")
     return out
@@ -525,19 +536,21 @@ def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor,
     """Token rows k / v [B,KVH,S,Dh] into units [unit0, unit0 + ceil(S / 16)) of a 4-bit record ``rec`` =
     (rec_k, rec_v), uint8 [B,KVH,units,10*Dh] on the device or in pinned host memory; a new device record
     of just these rows when None (see hga_kv4_pack).  Returns the record."""
-    _require_cuda(k, v)
+    if not (k.is_cuda and v.is_cuda):
+        _require_cuda(k, v)
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _lib.DTYPE_CODE:
         raise _lib.HgaError("kv4_pack: k and v must be [B,KVH,S,Dh] tensors of one shape and type (fp32 / bf16 / fp16)")
     B, KVH, S, Dh = k.shape
     units = -(-S // KV4_UNIT)
     if rec is None:
-        rec_k = torch.empty(B, KVH, unit0 + units, 10 * Dh, device=k.device, dtype=torch.uint8)
+        cap = unit0 + units
+        rec_k = k.new_empty((B, KVH, cap, 10 * Dh), dtype=torch.uint8)
         rec_v = torch.empty_like(rec_k)
     else:
         rec_k, rec_v = rec
-    cap = _kv4_rec("kv4_pack", rec_k, B, KVH, Dh)
-    if _kv4_rec("kv4_pack", rec_v, B, KVH, Dh) != cap:
-        raise _lib.HgaError("kv4_pack: rec_k and rec_v differ in capacity")
+        cap = _kv4_rec("kv4_pack", rec_k, B, KVH, Dh)
+        if _kv4_rec("kv4_pack", rec_v, B, KVH, Dh) != cap:
+            raise _lib.HgaError("kv4_pack: rec_k and rec_v differ in capacity")
     if k.numel() == 0:
         return rec_k, rec_v
     k, v = _kv4_rows(k), _kv4_rows(v)
@@ -564,6 +577,8 @@ def kv4_unpack(rec_k: torch.Tensor, rec_v: torch.Tensor, seq_len: int, dtype: to
     if _kv4_rec("kv4_unpack", rec_v, B, KVH, Dh) != cap:
         raise _lib.HgaError("kv4_unpack: rec_k and rec_v differ in capacity")
     dev = rec_k.device if device is None else torch.device(device)
+    if dev.index is None and dev.type == "cuda":
+        dev = torch.device("cuda", torch.cuda.current_device())
     if dev.type != "cuda":
         raise _lib.HgaError("hga ops run on CUDA tensors only (no CPU fallback): give kv4_unpack a CUDA device")
     k = torch.empty(B, KVH, seq_len, Dh, device=dev, dtype=dtype)
@@ -580,32 +595,36 @@ def attend_decode_kv4(p: HgaParams, q: torch.Tensor, seq_pos: torch.Tensor, hot_
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one decode block q [B,H,L,Dh] over the slot windows hot_* (hot_mode 1's layout) and the
     opened groups of a 4-bit record (see hga_attend_decode_kv4).  Returns [B,H,L,Dh]."""
-    _require_cuda(q, seq_pos, hot_k, hot_v, open_gid, open_t0)
+    idx = q.get_device()
+    for t in (seq_pos, hot_k, hot_v, open_gid, open_t0):
+        if t.get_device() != idx or idx < 0:
+            _require_cuda(q, seq_pos, hot_k, hot_v, open_gid, open_t0)
+            raise _lib.HgaError("attend_decode_kv4: tensors on different devices")
     if not q.is_contiguous():
         q = q.contiguous()
     B, H, L, Dh = q.shape
-    if (B, H, Dh) != (p.batch, p.nhead, p.head_dim) or _lib.DTYPE_CODE.get(q.dtype) != p.dtype:
-        raise _lib.HgaError(f"attend_decode_kv4: q {tuple(q.shape)} {q.dtype} does not fit the layer's parameters")
-    if hot_k.dtype != q.dtype or hot_v.dtype != q.dtype or hot_k.shape != hot_v.shape:
-        raise _lib.HgaError("attend_decode_kv4: hot_k / hot_v must have q's type and one shape")
-    if (seq_pos.dtype != torch.int32 or open_gid.dtype != torch.int32 or open_t0.dtype != torch.int32
-            or seq_pos.numel() != B or open_gid.shape != open_t0.shape or tuple(open_gid.shape[:2]) != (B, H)):
+    dtype = q.dtype
+    if B != p.batch or H != p.nhead or Dh != p.head_dim or _lib.DTYPE_CODE.get(dtype) != p.dtype:
+        raise _lib.HgaError(f"attend_decode_kv4: q {tuple(q.shape)} {dtype} does not fit the layer's parameters")
+    KVH = p.kv_heads
+    if (hot_k.dtype != dtype or hot_v.dtype != dtype or hot_k.shape != hot_v.shape or hot_k.shape[1] != KVH
+            or hot_k.stride() != hot_v.stride()):
+        raise _lib.HgaError("attend_decode_kv4: hot_k / hot_v must have q's type, [B,KVH,rows,Dh] and one layout")
+    i32 = torch.int32
+    if (seq_pos.dtype != i32 or open_gid.dtype != i32 or open_t0.dtype != i32 or seq_pos.numel() != B
+            or open_gid.shape != open_t0.shape or open_gid.shape[:2] != (B, H)):
         raise _lib.HgaError("attend_decode_kv4: seq_pos [B] and open_gid / open_t0 [B,H,Kg] must be int32")
     if not open_gid.is_contiguous() or not open_t0.is_contiguous():
         open_gid, open_t0 = open_gid.contiguous(), open_t0.contiguous()
-    KVH = p.kv_heads
     cap = _kv4_rec("attend_decode_kv4", rec_k, B, KVH, Dh)
-    if _kv4_rec("attend_decode_kv4", rec_v, B, KVH, Dh) != cap:
+    if rec_v.shape != rec_k.shape or _kv4_rec("attend_decode_kv4", rec_v, B, KVH, Dh) != cap:
         raise _lib.HgaError("attend_decode_kv4: rec_k and rec_v differ in capacity")
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+    elif out.shape != q.shape or out.dtype != dtype or not out.is_contiguous():
         raise _lib.HgaError("attend_decode_kv4: out must be contiguous, of q's shape and type")
-    hot_cap = kv_cap_of(hot_k)
-    if kv_cap_of(hot_v) != hot_cap:
-        raise _lib.HgaError("attend_decode_kv4: hot_k and hot_v must share one capacity layout")
-    rc = lib().hga_attend_decode_kv4(ctypes_params(p), L, q.data_ptr(), seq_pos.data_ptr(), hot_k.data_ptr(),
-                                     hot_v.data_ptr(), hot_cap, rec_k.data_ptr(), rec_v.data_ptr(), cap,
+    rc = lib().hga_attend_decode_kv4(ctypes.byref(p), L, q.data_ptr(), seq_pos.data_ptr(), hot_k.data_ptr(),
+                                     hot_v.data_ptr(), kv_cap_of(hot_k), rec_k.data_ptr(), rec_v.data_ptr(), cap,
                                      open_gid.data_ptr(), open_t0.data_ptr(), open_gid.shape[2], out.data_ptr(),
                                      stream_ptr(q.device))
     if rc:
