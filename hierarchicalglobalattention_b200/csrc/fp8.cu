@@ -103,9 +103,20 @@ __global__ void __launch_bounds__(256) fp8_realign_kernel(const uint8_t* __restr
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / per, c = (i - r * per) * 16;
     uint32_t w[4] = {0, 0, 0, 0};
+    const uint8_t* p = src + r * src_stride + c;
+    const int sh = (int)((uintptr_t)p & 3);
+    if (c - sh >= 0 && c + 20 <= k) {  // five aligned words, all inside the row
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p - sh);
+      uint32_t v[5];
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (c + e < k) w[e >> 2] |= (uint32_t)src[r * src_stride + c + e] << (8 * (e & 3));
+      for (int e = 0; e < 5; ++e) v[e] = q[e];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = __funnelshift_r(v[e], v[e + 1], 8 * sh);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (c + e < k) w[e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
+    }
     dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int c = 0; c < COLS; c += PC) {
         if (n0 + c >= a.n || m0 >= a.m) break;  // warp-uniform
         unsigned char* stg = stage + ((c / PC) & 1) * 4096;
-        if (a.tma_out) {
+        if (PAIR == 2 || a.tma_out) {
           if (lane == 0) bulk_wait_read1();  // the store before the last has been read out
           __syncwarp();
         }
@@ -302,23 +302,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               w[2 * e + 1] = __float_as_uint(hi);
             }
           }
-          if (a.tma_out) {
-            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          } else if (row < a.m) {
-            T* o = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + n0 + c + j * (16 / (int)sizeof(T));
-            const T* v = reinterpret_cast<const T*>(w);
-#pragma unroll
-            for (int e = 0; e < 16 / (int)sizeof(T); ++e)
-              if (n0 + c + j * (16 / (int)sizeof(T)) + e < a.n) o[e] = v[e];
-          }
+          *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        if (a.tma_out) {
+        if (PAIR == 2 || a.tma_out) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
             tma_store_2d(&tm_o, stg, n0 + c, m0);
             bulk_commit();
           }
+        } else {
+          // rows off the 16-byte grid: whole rows of the piece, neighbouring lanes neighbouring columns
+          __syncwarp();
+          const int rows = a.m - m0 < 32 ? a.m - m0 : 32;
+#pragma unroll
+          for (int h = 0; h < PC; h += 32) {
+            const int at = (h + lane) * (int)sizeof(T);
+            if (n0 + c + h + lane >= a.n) break;
+            T* o = static_cast<T*>(a.out) + (int64_t)m0 * a.out_stride + n0 + c + h + lane;
+            for (int r = 0; r < rows; ++r, o += a.out_stride)
+              *o = *reinterpret_cast<const T*>(stg + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+          }
+          __syncwarp();
         }
       }
     }
@@ -336,6 +341,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
+static bool rows_on_grid(const void* p, int64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % 16 == 0; }
+
 template <typename T, int BN, int PAIR, int STAGES>
 static cudaError_t tiles_t(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
                            const void* w, int64_t w_stride, cudaStream_t st) {
@@ -347,7 +354,7 @@ static cudaError_t tiles_t(const Fp8Linear& a, const void* q, int64_t q_stride, 
       !make_map_typed(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, 2, dw, sw, bw, CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   const int64_t ostr = a.out_stride * (int64_t)sizeof(T);
-  const bool tma_out = ((uintptr_t)a.out & 15) == 0 && ostr % 16 == 0;
+  const bool tma_out = rows_on_grid(a.out, ostr);
   mo = mx;
   if (tma_out) {
     const cuuint64_t d[2] = {(cuuint64_t)a.n, (cuuint64_t)a.m}, s[1] = {(cuuint64_t)ostr};
@@ -388,7 +395,9 @@ static cudaError_t tiles_n(const Fp8Linear& a, const void* q, int64_t q_stride, 
   // 256 x 256 tiles of CTA pairs where they fill the GPU: a pair reads half as many bytes per product as
   // 128 x 128 tiles, and the loads from L2 are what bounds them
   const int64_t pairs = (a.m + 255) / 256 * ((a.n + 255) / 256);
-  if (pairs >= 74) return tiles_t<T, 256, 2, 5>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
+  // (their results leave by TMA only: the plain stores' registers would spill the sums)
+  if (pairs >= 74 && rows_on_grid(a.out, a.out_stride * (int64_t)sizeof(T)))
+    return tiles_t<T, 256, 2, 5>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
   return tiles_t<T, 128, 1, 4>(a, q, q_stride, xs, xs_stride, w, w_stride, st);
 }
 
