@@ -20,7 +20,7 @@ namespace hga {
 constexpr int kQuantWarps = 8;
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQuantWarps * 32) fp8_quantize_kernel(const T* __restrict__ x, int64_t x_stride,
+__global__ void __launch_bounds__(kQuantWarps * 32, 5) fp8_quantize_kernel(const T* __restrict__ x, int64_t x_stride,
                                                                         int64_t m, int64_t k, int kb, int segs,
                                                                         uint8_t* __restrict__ q, int64_t q_stride,
                                                                         int64_t q_cols, float* __restrict__ scale,

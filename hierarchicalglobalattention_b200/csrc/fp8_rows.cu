@@ -278,12 +278,12 @@ __global__ void __launch_bounds__(rows_threads(FUSED))
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kCols));
 }
 
-// CTAs along the channels: enough to give every SM about two CTAs' worth of weight, at least two
+// CTAs along the channels: as many as are resident at once (two an SM less what clusters leave empty), at least two
 // blocks each, at most 8 (a portable cluster) and kMaxSlice blocks a CTA.
 static int rows_splits(int64_t m, int64_t n, int64_t kb, int tn) {
   const int64_t tiles = (n + 127) / 128 * ((m + tn - 1) / tn);
   int s = 1;
-  while (s < 8 && ((tiles * s * 2 <= 148 * 2 && kb >= 4 * s) || kb > (int64_t)s * kMaxSlice)) s *= 2;
+  while (s < 8 && ((tiles * s * 2 <= 264 && kb >= 4 * s) || kb > (int64_t)s * kMaxSlice)) s *= 2;
   return s;
 }
 

@@ -18,7 +18,7 @@
 // up to 1 % of a score (the instruction truncates its sums relative to their largest term), and in the
 // output, whose sum runs over all keys, a bf16 ulp.
 //
-// Units are dealt to the 8 warps of the `splits` CTAs of a cluster (windows and the active chunk first,
+// Units are dealt to the warps of the `splits` CTAs of a cluster (windows and the active chunk first,
 // then the union); every warp keeps its own online softmax and copies its next units with cp.async (plain
 // loads for records in pinned host memory, where asynchronous copies are slower).  Warps join in shared
 // memory, CTAs through distributed shared memory, in a fixed order: no atomics on results, one launch.
@@ -36,7 +36,9 @@ namespace kv4 {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 8;
+// warps of a CTA and CTAs an SM: with 8 columns a warp's state fits 128 registers, with 16 it takes 168
+__host__ __device__ constexpr int warps_of(int nt) { return nt == 1 ? 8 : 4; }
+__host__ __device__ constexpr int ctas_of(int nt) { return nt == 1 ? 2 : 3; }
 constexpr int kStages = 4;          // record units in flight per warp
 constexpr int kNever = 255;         // t0 of a (unit, head) that does not see the unit
 
@@ -145,6 +147,7 @@ __device__ __forceinline__ uint4 load16(const void* p) {
 
 // Shared memory: the warps' copy buffers (afterwards their partial results), then the union's tables.
 template <int DH, int NT> struct Layout {
+  static constexpr int kWarps = warps_of(NT);
   static constexpr int kOut = DH * 8 * NT * 4;                       // one partial O^T, fp32
   static constexpr int kRing = kWarps * Buf<DH>::kWarp;
   static constexpr int kPart = kWarps * kOut + 8 * NT * (DH + 4) * 4 + (kWarps + 1) * 2 * 8 * NT * 4;
@@ -160,9 +163,10 @@ static size_t table_bytes(int hr, int Kg, int hash_bits) {
 }
 
 template <typename T, int DH, int NT>
-__global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma_kernel(const hga_params p, const Args a) {
+__global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma_kernel(const hga_params p, const Args a) {
   using H = Half2<T>;
   using LY = Layout<DH, NT>;
+  constexpr int kWarps = LY::kWarps;
   constexpr int KS = DH / 16, NB = DH / 32, COLS = 8 * NT;
   // what the keys' codes have in the products besides themselves: 8 off (n - 8), or 128 on (bf16 keeps it:
   // 128 sum q is taken off in fp32 with an error of 1e-5 of a score)
@@ -181,11 +185,11 @@ __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 2 : 1)) attend_kv4_mma
   int* misc = reinterpret_cast<int*>(smem + LY::kMisc);
 
   cg::cluster_group cl = cg::this_cluster();
-  // the first entries of the heads' lists (one or two a thread: all of them for 64 groups and 8 heads), asked
+  // the first entries of the heads' lists (all of them for 64 groups and 8 heads), asked
   // for before anything waits for the sequence's position
   const int N = hr * Kg, hsize = 1 << a.hash_bits;
   const size_t list0 = ((size_t)b * p.nhead + h0) * Kg;
-  constexpr int kEarly = 2;
+  constexpr int kEarly = 512 / (kWarps * 32);
   int e_gid[kEarly], e_t0[kEarly];
 #pragma unroll
   for (int j = 0; j < kEarly; ++j) {
@@ -794,7 +798,7 @@ static cudaError_t launch_t(const hga_params& p, Args a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.splits, p.batch * p.kv_heads, (unsigned)z);
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(warps_of(NT) * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -825,9 +829,10 @@ cudaError_t launch_attend_kv4_mma(const hga_params& p, int L, const void* q, con
   const int cols = (a.rep < 8 ? a.rep : 8) * L;
   const bool wide = cols > 8;
   const int64_t ctas = (int64_t)p.batch * p.kv_heads * ((a.rep + 7) / 8) * ((cols + (wide ? 15 : 7)) / (wide ? 16 : 8));
-  // CTAs per tile: up to two CTAs an SM, at most 8 (a portable cluster)
-  a.splits = 1;
-  while (a.splits < 8 && ctas * a.splits * 2 <= 148 * 2) a.splits *= 2;
+  // CTAs per tile: as many as are resident at once, at most 8 (a portable cluster).  Clusters of 4 to 8 leave
+  // about a tenth of the places empty (33 of 8 CTAs fit where 37 would): a 36th of 8 would wait for a second round.
+  const int64_t room = 132 * kv4::ctas_of(wide ? 2 : 1);
+  a.splits = (int)(room / ctas < 1 ? 1 : room / ctas > 8 ? 8 : room / ctas);
 #define HGA_KV4_L(TT)                                                                              \
   if (p.head_dim == 128) return wide ? kv4::launch_t<TT, 128, 2>(p, a, st) : kv4::launch_t<TT, 128, 1>(p, a, st); \
   return wide ? kv4::launch_t<TT, 64, 2>(p, a, st) : kv4::launch_t<TT, 64, 1>(p, a, st);
