@@ -15,8 +15,10 @@ namespace hga {
 // A warp takes 8 neighbouring blocks of a row, two at a time (16 lanes a block, 8 channels a lane), their
 // four loads in flight together.  The four rounds' scales and reciprocals are worked out side by side, one
 // round a lane, and handed out by shuffles: computed per round they were a third of the instructions.
-// Bound by HBM (2 bytes read and 1 written per 16-bit channel) and nearly so by issue.  VEC: rows and base are
-// 16-byte aligned (8-byte for q).
+// Bound by HBM (2 bytes read and 1 written per 16-bit channel) and nearly so by issue: 32768 x 4096 bf16 in 75 us,
+// 5.4 TB/s, 83 % of the measured copy (plain divisions, a scale a block and one block in flight a warp: 160 us).
+// Five CTAs an SM: 78 us with four, 80 with six (its registers spill).  VEC: rows and base are 16-byte
+// aligned (8-byte for q).
 constexpr int kQuantWarps = 8;
 
 template <typename T, bool VEC>

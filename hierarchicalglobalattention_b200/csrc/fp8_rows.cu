@@ -10,6 +10,9 @@
 //   warps 2-5  then one feature a thread: sum[token] += D * (ws * xs[token]) per block
 // FUSED saves the quantisation's launch and its round trip through memory; past some 64 blocks a CTA its
 // repetition in every CTA costs more than that (16 x 8192 into 8192 features: 22.3 us against 14.2).
+// One token of 2048 channels into 5120 features: 7.6 us (the launch of a cluster and the chain of loads, product
+// and join bound it; the weight alone is 1.6 us of HBM); 16 rows of 8192 channels, already quantised, into 8192
+// features: 11.8 us, 5.7 TB/s of weight.
 #include <cooperative_groups.h>
 
 #include "fp8_common.cuh"

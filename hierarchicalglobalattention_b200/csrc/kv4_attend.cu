@@ -22,7 +22,10 @@
 // then the union); every warp keeps its own online softmax and copies its next units with cp.async (plain
 // loads for records in pinned host memory, where asynchronous copies are slower).  Warps join in shared
 // memory, CTAs through distributed shared memory, in a fixed order: no atomics on results, one launch.
-// Bound by HBM when many sequences decode, by latency for one.
+// One token for each of 16 sequences of 32768 (32 heads over 4): 26 us for 63 MB (2.4 TB/s); issue of the
+// decoding bounds it there (some 400 instructions a unit and warp, 39 % of the SMs' issue), set-up and the two
+// cluster barriers (10 us together) for one sequence: 11.5 us at 4096 tokens.  One pass over keys per query head
+// with plain FMAs took 566 and 398 us.
 #include <cooperative_groups.h>
 
 #include "fp32x2.cuh"
