@@ -71,9 +71,7 @@ class Kv4CacheStore(RamKVCacheStore):
         return st.token_k, st.token_v
 
     def cold_buffers(self, layer: int):
-        # a decode block: the prefill's exact rows are no longer needed, and new rows enter the record when
-        # their chunk closes
-        self._seed_rows.pop(layer, None)
+        # new rows enter the record when their chunk closes
         return None, None
 
     def adopt_tokens(self, layer, token_k, token_v) -> None:
@@ -88,7 +86,8 @@ class Kv4CacheStore(RamKVCacheStore):
         """Pack rows [row0, row0 + L); row0 a multiple of 16."""
         if row0 % ops.KV4_UNIT:
             raise ValueError("rows enter the 4-bit record in whole 16-token units")
-        self._seed_rows[layer] = (token_k, token_v)
+        if row0 == 0:
+            self._seed_rows[layer] = (token_k, token_v)
         ops.kv4_pack(token_k, token_v, self.record(layer), unit0=row0 // ops.KV4_UNIT)
 
     def on_chunk_closed(self, layer: int, n: int, row: Optional[int] = None) -> None:
@@ -115,6 +114,8 @@ class Kv4CacheStore(RamKVCacheStore):
             k_act, v_act = self.active_rows(layer, n)
             k_act[bs, :, :rem].copy_(k[bs, :, n * C:seq_len])
             v_act[bs, :, :rem].copy_(v[bs, :, n * C:seq_len])
+        if row is None or row == self.B - 1:
+            del self._seed_rows[layer]
 
     # -- the VRAM bank, on packed groups ---------------------------------------------------------
     def _group_bytes(self) -> int:

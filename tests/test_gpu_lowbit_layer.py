@@ -73,6 +73,21 @@ def test_decode_through_the_4bit_store(cuda):
     assert other.store.cache_hits > 0 and other.store.cache_misses > 0
 
 
+def test_a_seeded_store_lets_go_of_the_exact_rows(cuda):
+    import weakref
+    g = _inputs(cuda, 2, 300)
+    for mixed in (False, True):
+        router = _kv4(cuda, 2)
+        k, v = g["k_rope"][:, :, :300].clone(), g["v"][:, :, :300].clone()
+        refs = weakref.ref(k), weakref.ref(v)
+        if mixed:
+            router.seed_mixed(0, k, g["k_raw"][:, :, :300], v, [300, 130])
+        else:
+            router.seed(0, k, g["k_raw"][:, :, :300], v)
+        del k, v
+        assert refs[0]() is None and refs[1]() is None
+
+
 def test_graph_and_reset_equal_eager(cuda):
     from hierarchicalglobalattention_b200.decode_graph import DecodeStepGraph
     B, S0, steps = 2, 500, 70
