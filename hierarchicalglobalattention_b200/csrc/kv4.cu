@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kPortWarps * 32) attend_kv4_kernel(
   for (int j = 0; j < Kg; ++j) {
     const int gid = open_gid[bh * Kg + j], t0 = open_t0[bh * Kg + j];
     if (gid < 0 || t0 < 0) continue;
-    if ((int64_t)(gid + 1) * U > unit_cap) {
+    if (((int64_t)gid + 1) * U > unit_cap) {
       if (tid == 0) atomicCAS(&g_kv4_error, 0, kErrBoundsAttendKv4);
       continue;
     }
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kPortWarps * 32) attend_kv4_kernel(
     const int r = warp * 2 + i;
     if (r >= nrows) continue;
 #pragma unroll
-    for (int d = 0; d < VD; ++d) o_base[(size_t)r * DH + lane + 32 * d] = Num<T>::from_f(l[i] == 0.f ? 0.f : o[i][d] / l[i]);
+    for (int d = 0; d < VD; ++d) o_base[(size_t)r * DH + lane + 32 * d] = Num<T>::from_f(o[i][d] / l[i]);
   }
 }
 

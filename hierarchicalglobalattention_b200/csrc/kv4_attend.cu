@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
   auto insert = [&](int i, int gid, int t0) {
     int s = -1;
     if (gid >= 0 && t0 >= 0 && t0 <= t_last) {
-      if ((int64_t)(gid + 1) * U > a.unit_cap) {
+      if (((int64_t)gid + 1) * U > a.unit_cap) {
         atomicCAS(&g_kv4_mma_error, 0, kErrBoundsAttendKv4);
       } else {
         s = (int)((uint32_t)gid * 2654435761u >> (32 - a.hash_bits));
@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[nt][e] = vis[nt] >> e & 1 ? ex2(s[nt][e] - m[nt][e & 1]) : 0.f;
+        // a maximum of -infinity: only such scores so far, whose weight is 0 (a NaN stays one)
+        s[nt][e] = vis[nt] >> e & 1 ? ex2(s[nt][e] - (m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1])) : 0.f;
         l[nt][e & 1] += s[nt][e];
       }
   };
@@ -779,7 +780,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
       acc += f * vr[r];
     }
     const int x = x0 + col;
-    out[(((size_t)b * p.nhead + h0 + x % hr) * L + x / hr) * DH + ch] = Num<T>::from_f(sum == 0.f ? 0.f : acc / sum);
+    out[(((size_t)b * p.nhead + h0 + x % hr) * L + x / hr) * DH + ch] = Num<T>::from_f(acc / sum);
   }
   if (a.splits > 1) cl.sync();  // no CTA leaves while another still reads its sums
 }

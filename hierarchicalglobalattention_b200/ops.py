@@ -482,10 +482,15 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     elif out.dtype != out_dtype or out.shape != (*shape[:-1], N) or not out.is_contiguous():
         raise _lib.HgaError("fp8_linear: out must be a contiguous [..., N] tensor of the result's type")
     h = lib()
-    xp, wp, xst, wst = r.data_ptr(), w.data_ptr(), r.stride(0), w.stride(0)
-    xst, wst, sst = xst if xst > K else K, wst if wst > K else K, w_scale.stride(0)
-    call = (M, N, K, code, xp, xst, None if xs is None else xs.data_ptr(), wp, wst, w_scale.data_ptr(),
-            sst if sst > KB else KB, None if bias is None else bias.data_ptr(), ocode, out.data_ptr(), N)
+    xp, wp, xst, wst, sst = r.data_ptr(), w.data_ptr(), r.stride(0), w.stride(0), w_scale.stride(0)
+    if xst < K:
+        xst = K                 # a single row's stride is free
+    if wst < K or sst < KB:     # broadcast or overlapping rows
+        if (wst < K and N > 1) or (sst < KB and NB > 1):
+            raise _lib.HgaError("fp8_linear: rows of w and w_scale must not overlap (call contiguous() on broadcast ones)")
+        wst, sst = max(wst, K), max(sst, KB)
+    call = (M, N, K, code, xp, xst, None if xs is None else xs.data_ptr(), wp, wst, w_scale.data_ptr(), sst,
+            None if bias is None else bias.data_ptr(), ocode, out.data_ptr(), N)
     stream = stream_ptr(dev)
     # few rows mostly need no workspace: asked for only when the call says so
     if M <= _FP8_FEW_ROWS and h.hga_fp8_linear(*call, None, 0, stream) == 0:
@@ -509,26 +514,33 @@ def kv4_unit_bytes(head_dim: int) -> int:
     return 10 * head_dim
 
 
-def _kv4_rec(name: str, rec: torch.Tensor, B: int, KVH: int, Dh: int) -> int:
-    """Units allocated per (sequence, KV head) of a record [B, KVH, units, 10 * Dh]."""
+def _kv4_rec(name: str, rec: torch.Tensor, B: int, KVH: int, Dh: int, device: int) -> int:
+    """Units allocated per (sequence, KV head) of a record [B, KVH, units, 10 * Dh] on the device or pinned."""
     shape = rec.shape
     if (rec.dtype != torch.uint8 or len(shape) != 4 or shape[0] != B or shape[1] != KVH or shape[3] != 10 * Dh
             or not rec.is_contiguous()):
         raise _lib.HgaError(f"{name}: a record is a contiguous uint8 [B, KVH, units, 10 * Dh] tensor; got {rec.dtype} "
                             f"{tuple(shape)} for B={B}, KVH={KVH}, Dh={Dh}")
-    if not rec.is_cuda and not rec.is_pinned():
-        raise _lib.HgaError(f"{name}: a record in host memory must be pinned")
+    idx = rec.get_device()
+    if idx != device and (idx >= 0 or not rec.is_pinned()):
+        raise _lib.HgaError(f"{name}: a record in host memory must be pinned" if idx < 0 else
+                            f"{name}: tensors on different devices")
     return shape[2]
 
 
-def _kv4_rows(t: torch.Tensor) -> torch.Tensor:
-    """K/V rows as a row-slice of a contiguous [B,KVH,cap,Dh] buffer (copied when they are laid out otherwise)."""
-    if t.is_contiguous() and not t.data_ptr() & 15:
-        return t
+def _kv4_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """K/V rows [B,KVH,S,Dh] as a row-slice of a contiguous [B,KVH,cap,Dh] buffer, and that buffer's cap (copied
+    when they are laid out otherwise)."""
     B, KVH, S, Dh = t.shape
-    s0, s1, s2, s3 = t.stride()
-    ok = s3 == 1 and s2 == Dh and s1 % Dh == 0 and s1 >= S * Dh and s0 == KVH * s1 and not t.data_ptr() & 15
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    if not t.data_ptr() & 15:
+        if t.is_contiguous():       # strides of dimensions of size one are free
+            return t, S
+        s0, s1, s2, s3 = t.stride()
+        if KVH == 1:
+            s1 = s0 if B > 1 else S * Dh
+        if s3 == 1 and (s2 == Dh or S == 1) and s1 % Dh == 0 and s1 >= S * Dh and (B == 1 or s0 == KVH * s1):
+            return t, s1 // Dh
+    return t.clone(memory_format=torch.contiguous_format), S
 
 
 def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
@@ -541,6 +553,9 @@ def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor,
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _lib.DTYPE_CODE:
         raise _lib.HgaError("kv4_pack: k and v must be [B,KVH,S,Dh] tensors of one shape and type (fp32 / bf16 / fp16)")
     B, KVH, S, Dh = k.shape
+    idx = k.get_device()
+    if v.get_device() != idx:
+        raise _lib.HgaError("kv4_pack: tensors on different devices")
     units = -(-S // KV4_UNIT)
     if rec is None:
         cap = unit0 + units
@@ -548,15 +563,15 @@ def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor,
         rec_v = torch.empty_like(rec_k)
     else:
         rec_k, rec_v = rec
-        cap = _kv4_rec("kv4_pack", rec_k, B, KVH, Dh)
-        if _kv4_rec("kv4_pack", rec_v, B, KVH, Dh) != cap:
+        cap = _kv4_rec("kv4_pack", rec_k, B, KVH, Dh, idx)
+        if _kv4_rec("kv4_pack", rec_v, B, KVH, Dh, idx) != cap:
             raise _lib.HgaError("kv4_pack: rec_k and rec_v differ in capacity")
     if k.numel() == 0:
         return rec_k, rec_v
-    k, v = _kv4_rows(k), _kv4_rows(v)
-    if k.stride(1) != v.stride(1):
-        k, v = k.contiguous(), v.contiguous()
-    rc = lib().hga_kv4_pack(_lib.DTYPE_CODE[k.dtype], Dh, B * KVH, S, k.data_ptr(), v.data_ptr(), k.stride(1) // Dh,
+    (k, kv_cap), (v, v_cap) = _kv4_rows(k), _kv4_rows(v)
+    if kv_cap != v_cap:
+        k, v, kv_cap = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format), S
+    rc = lib().hga_kv4_pack(_lib.DTYPE_CODE[k.dtype], Dh, B * KVH, S, k.data_ptr(), v.data_ptr(), kv_cap,
                             rec_k.data_ptr(), rec_v.data_ptr(), cap, unit0, stream_ptr(k.device))
     if rc:
         check(rc, "hga_kv4_pack")
@@ -573,14 +588,14 @@ def kv4_unpack(rec_k: torch.Tensor, rec_v: torch.Tensor, seq_len: int, dtype: to
         raise _lib.HgaError("kv4_unpack: a record is a uint8 [B, KVH, units, 10 * Dh] tensor")
     B, KVH, _, nb = rec_k.shape
     Dh = nb // 10
-    cap = _kv4_rec("kv4_unpack", rec_k, B, KVH, Dh)
-    if _kv4_rec("kv4_unpack", rec_v, B, KVH, Dh) != cap:
-        raise _lib.HgaError("kv4_unpack: rec_k and rec_v differ in capacity")
     dev = rec_k.device if device is None else torch.device(device)
-    if dev.index is None and dev.type == "cuda":
-        dev = torch.device("cuda", torch.cuda.current_device())
     if dev.type != "cuda":
         raise _lib.HgaError("hga ops run on CUDA tensors only (no CPU fallback): give kv4_unpack a CUDA device")
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    cap = _kv4_rec("kv4_unpack", rec_k, B, KVH, Dh, dev.index)
+    if _kv4_rec("kv4_unpack", rec_v, B, KVH, Dh, dev.index) != cap:
+        raise _lib.HgaError("kv4_unpack: rec_k and rec_v differ in capacity")
     k = torch.empty(B, KVH, seq_len, Dh, device=dev, dtype=dtype)
     v = torch.empty_like(k)
     rc = lib().hga_kv4_unpack(_lib.DTYPE_CODE[dtype], Dh, B * KVH, seq_len, rec_k.data_ptr(), rec_v.data_ptr(), cap,
@@ -607,21 +622,22 @@ def attend_decode_kv4(p: HgaParams, q: torch.Tensor, seq_pos: torch.Tensor, hot_
     if B != p.batch or H != p.nhead or Dh != p.head_dim or _lib.DTYPE_CODE.get(dtype) != p.dtype:
         raise _lib.HgaError(f"attend_decode_kv4: q {tuple(q.shape)} {dtype} does not fit the layer's parameters")
     KVH = p.kv_heads
-    if (hot_k.dtype != dtype or hot_v.dtype != dtype or hot_k.shape != hot_v.shape or hot_k.shape[1] != KVH
-            or hot_k.stride() != hot_v.stride()):
+    hot = hot_k.shape
+    if (hot_k.dtype != dtype or hot_v.dtype != dtype or hot != hot_v.shape or len(hot) != 4 or hot[0] != B
+            or hot[1] != KVH or hot[3] != Dh or hot_k.stride() != hot_v.stride()):
         raise _lib.HgaError("attend_decode_kv4: hot_k / hot_v must have q's type, [B,KVH,rows,Dh] and one layout")
     i32 = torch.int32
     if (seq_pos.dtype != i32 or open_gid.dtype != i32 or open_t0.dtype != i32 or seq_pos.numel() != B
             or open_gid.shape != open_t0.shape or open_gid.shape[:2] != (B, H)):
         raise _lib.HgaError("attend_decode_kv4: seq_pos [B] and open_gid / open_t0 [B,H,Kg] must be int32")
-    if not open_gid.is_contiguous() or not open_t0.is_contiguous():
-        open_gid, open_t0 = open_gid.contiguous(), open_t0.contiguous()
-    cap = _kv4_rec("attend_decode_kv4", rec_k, B, KVH, Dh)
-    if rec_v.shape != rec_k.shape or _kv4_rec("attend_decode_kv4", rec_v, B, KVH, Dh) != cap:
+    if not (open_gid.is_contiguous() and open_t0.is_contiguous() and seq_pos.is_contiguous()):
+        open_gid, open_t0, seq_pos = open_gid.contiguous(), open_t0.contiguous(), seq_pos.contiguous()
+    cap = _kv4_rec("attend_decode_kv4", rec_k, B, KVH, Dh, idx)
+    if _kv4_rec("attend_decode_kv4", rec_v, B, KVH, Dh, idx) != cap:
         raise _lib.HgaError("attend_decode_kv4: rec_k and rec_v differ in capacity")
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != dtype or not out.is_contiguous():
+    elif out.shape != q.shape or out.dtype != dtype or out.get_device() != idx or not out.is_contiguous():
         raise _lib.HgaError("attend_decode_kv4: out must be contiguous, of q's shape and type")
     rc = lib().hga_attend_decode_kv4(ctypes.byref(p), L, q.data_ptr(), seq_pos.data_ptr(), hot_k.data_ptr(),
                                      hot_v.data_ptr(), kv_cap_of(hot_k), rec_k.data_ptr(), rec_v.data_ptr(), cap,

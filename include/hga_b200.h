@@ -298,7 +298,8 @@ int hga_kv4_unpack(int32_t dtype, int32_t head_dim, int64_t heads, int64_t rows,
 /* hga_attend_decode_kv4: hga_attend_decode with hot_mode 1 whose opened groups come from a 4-bit record
  * (unit g * (group_size / 16) is the first unit of group g; group_size a multiple of 16, rec_* device or
  * pinned host memory).  Windows and the active chunk are read from the slots in the cache's type.  Rows of the
- * slots and the record that a query row does not see do not count, whatever they hold. */
+ * slots and the record that a query row does not see do not count, whatever they hold.  A head's list names a
+ * group at most once. */
 int hga_attend_decode_kv4(const hga_params* p, int32_t L, const void* q, const int32_t* seq_pos, const void* hot_k,
                           const void* hot_v, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
                           const int32_t* open_gid, const int32_t* open_t0, int32_t Kg, void* out, cudaStream_t stream);

@@ -222,6 +222,12 @@ def test_refusals(cuda):
         ops.fp8_linear(x, w, ws, bias=torch.zeros(256, device=cuda))
     with pytest.raises(E, match="out"):
         ops.fp8_linear(x, w, ws, out=torch.zeros(4, 255, device=cuda, dtype=torch.bfloat16))
+    with pytest.raises(E, match="overlap"):
+        ops.fp8_linear(x, w[:1].expand(256, 384), ws)
+    with pytest.raises(E, match="overlap"):
+        ops.fp8_linear(x, w, ws[:1].expand(2, 3))
+    one = ops.fp8_linear(x + 1, w[:1].expand(1, 384), ws[:1].expand(1, 3))
+    assert torch.equal(one, ops.fp8_linear(x + 1, w[:1].clone(), ws[:1].clone()))
     with pytest.raises(E, match="CUDA"):
         ops.fp8_linear(x.cpu(), w, ws)
     with pytest.raises(E, match="x must be"):

@@ -301,6 +301,51 @@ def test_bounds_are_reported_not_read(cuda):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("Dh,dtype", [(128, torch.bfloat16), (64, torch.float16), (128, torch.float32)])
+def test_scores_of_minus_infinity(cuda, Dh, dtype):
+    """A key of -infinity against every query has weight 0, also where it is all that a unit shows."""
+    g = torch.Generator().manual_seed(19)
+    st = _state(g, 1, 8, 2, Dh, dtype, 64, 16, 1, 1, [640], 1, 6, cuda)
+    st["q"][..., 5] = 1.0
+    st["hk"][:, :, 2 * 64, 5] = -math.inf
+    _check(_run(st, cuda), st)
+
+
+def test_largest_group_number_is_out_of_bounds(cuda):
+    from hierarchicalglobalattention_b200 import _lib
+    g = torch.Generator().manual_seed(20)
+    for dtype in (torch.bfloat16, torch.float32):
+        st = _state(g, 1, 8, 1, 128, dtype, 64, 16, 1, 1, [700], 1, 8, cuda)
+        _lib.device_status()
+        st["gid"][0, 2, 0] = 2 ** 31 - 1
+        out = _run(st, cuda)
+        assert _lib.device_status() == 0x104
+        st["gid"][0, 2, 0] = -1
+        assert torch.equal(_run(st, cuda), out)
+
+
+@pytest.mark.parametrize("B", [1, 2])
+@pytest.mark.parametrize("S", [1, 40])
+def test_pack_one_kv_head_of_token_major_rows(cuda, B, S):
+    """[B,S,1,Dh] rows seen as [B,1,S,Dh]: contiguous, with free strides in the dimensions of size one."""
+    from hierarchicalglobalattention_b200 import ops
+    g = torch.Generator().manual_seed(21)
+    k, v = (t.to(cuda) for t in _kv(g, B, 1, 2 * S, 128, torch.bfloat16))
+    want = ops.kv4_pack(k[:, :, :S].contiguous(), v[:, :, :S].contiguous())
+    tk, tv = k[:, 0, :S].unsqueeze(2).contiguous().transpose(1, 2), v[:, 0, :S, None].transpose(1, 2)
+    for a, b in ((tk, tv), (tk, tk), (k[:, :, :S], tv), (k[:, :, :S], v[:, :, :S])):
+        got = ops.kv4_pack(a, b)
+        assert torch.equal(got[0], want[0]) and (b is tk or torch.equal(got[1], want[1]))
+
+
+def test_strided_positions(cuda):
+    g = torch.Generator().manual_seed(22)
+    st = _state(g, 2, 8, 1, 128, torch.bfloat16, 64, 16, 1, 1, [700, 300], 1, 8, cuda)
+    want = _run(st, cuda)
+    st["pos"] = torch.tensor([[700, 0], [300, 0]], dtype=torch.int32, device=cuda)[:, 0]
+    assert torch.equal(_run(st, cuda), want)
+
+
 def test_refusals(cuda):
     from hierarchicalglobalattention_b200 import _lib, ops
     g = torch.Generator().manual_seed(18)
@@ -323,6 +368,16 @@ def test_refusals(cuda):
         ops.attend_decode_kv4(
             st["p"], st["q"].half().to(cuda), st["pos"].to(cuda), st["hk"].to(cuda), st["hv"].to(cuda), *st["rec"],
             st["gid"].to(cuda), st["t0"].to(cuda))
+    for name in ("hk", "hv"):      # the slots of too few sequences, of another width
+        for bad in (st[name][:0], st[name][..., :64].contiguous()):
+            with pytest.raises(E, match="one layout"):
+                _run({**st, name: bad}, cuda)
+            with pytest.raises(E, match="one layout"):
+                _run({**st, "hk": bad, "hv": bad}, cuda)
+    dev = (st["q"].to(cuda), st["pos"].to(cuda), st["hk"].to(cuda), st["hv"].to(cuda), *st["rec"], st["gid"].to(cuda),
+           st["t0"].to(cuda))
+    with pytest.raises(E, match="out must be"):
+        ops.attend_decode_kv4(st["p"], *dev, out=torch.empty_like(st["q"]))
     st["gid"] = st["gid"].long()
     with pytest.raises(E, match="int32"):
         _run(st, cuda)
