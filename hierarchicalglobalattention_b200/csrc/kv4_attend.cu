@@ -1,7 +1,7 @@
 // Decode attention over the 4-bit record for 16-bit caches (head_dim 64 / 128), all query heads of a KV head
 // at once.
 //
-// A CTA serves up to 8 query heads of one KV head (x 8 * NT columns of (head, new row) pairs).  It forms the
+// A CTA serves up to 8 query heads of one KV head, 8 * NT columns of (head, new row) pairs.  It forms the
 // union of the groups those heads opened, so a group is read and decoded once for all of them, and works
 // in units of 16 keys on m16n8k16 matrix instructions with the keys as the 16 rows:
 //   S^T [16 keys][8 columns]  = K_unit Q^T           O^T [dims][8 columns] += V_unit^T P^T
@@ -24,7 +24,7 @@
 // memory, CTAs through distributed shared memory, in a fixed order: no atomics on results, one launch.
 // One token for each of 16 sequences of 32768 (32 heads over 4): 26 us for 63 MB (2.4 TB/s); issue of the
 // decoding bounds it there (some 400 instructions a unit and warp, 39 % of the SMs' issue), set-up and the two
-// cluster barriers (10 us together) for one sequence: 11.5 us at 4096 tokens.  One pass over keys per query head
+// cluster barriers (9 us together) for one sequence: 10.4 us at 4096 tokens.  One pass over keys per query head
 // with plain FMAs took 566 and 398 us.
 #include <cooperative_groups.h>
 
@@ -55,7 +55,7 @@ template <int DH> struct Buf {
 };
 
 struct Args {
-  int L, Kg, splits, rep, heads_blk, tiles, hash_bits, direct;
+  int L, Kg, splits, rep, hpc, tiles, hash_bits, direct;  // hpc: query heads of a CTA
   const void *q, *hot_k, *hot_v;
   const uint8_t *rec_k, *rec_v;
   const int32_t *seq_pos, *open_gid, *open_t0;
@@ -180,8 +180,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int rank = blockIdx.x, bk = blockIdx.y, b = bk / p.kv_heads, kvh = bk % p.kv_heads;
   const int hb = blockIdx.z / a.tiles, tile = blockIdx.z % a.tiles;
-  const int hr = a.rep - hb * 8 < 8 ? a.rep - hb * 8 : 8;            // heads of this CTA
-  const int h0 = kvh * a.rep + hb * 8;
+  const int hr = a.rep - hb * a.hpc < a.hpc ? a.rep - hb * a.hpc : a.hpc;  // heads of this CTA
+  const int h0 = kvh * a.rep + hb * a.hpc;
   const int x0 = tile * COLS, ncols = hr * a.L - x0 < COLS ? hr * a.L - x0 : COLS;
   const int C = p.chunk_size, U = p.group_size / kKv4Unit, L = a.L, Kg = a.Kg;
   const int kf = p.keep_first > 0 ? p.keep_first : 0, kl = p.keep_last > 0 ? p.keep_last : 0;
@@ -787,14 +787,13 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
 
 template <typename T, int DH, int NT>
 static cudaError_t launch_t(const hga_params& p, Args a, cudaStream_t st) {
-  const int hr = a.rep < 8 ? a.rep : 8;
-  a.heads_blk = (a.rep + 7) / 8;
+  const int hr = a.hpc, heads_blk = (a.rep + hr - 1) / hr;
   a.tiles = (hr * a.L + 8 * NT - 1) / (8 * NT);
   a.hash_bits = 5;
   while ((1 << a.hash_bits) < 2 * hr * a.Kg) ++a.hash_bits;
   const size_t smem = Layout<DH, NT>::kTables + table_bytes(hr, a.Kg, a.hash_bits);
   if (smem > 227 * 1024) return cudaErrorNotSupported;
-  const int64_t z = (int64_t)a.heads_blk * a.tiles;
+  const int64_t z = (int64_t)heads_blk * a.tiles;
   if (z > 65535 || (int64_t)p.batch * p.kv_heads > 65535) return cudaErrorNotSupported;
   auto kern = attend_kv4_mma_kernel<T, DH, NT>;
   static unsigned long long raised = 0;
@@ -830,9 +829,19 @@ cudaError_t launch_attend_kv4_mma(const hga_params& p, int L, const void* q, con
   cudaPointerAttributes pa;
   if (Kg > 0 && cudaPointerGetAttributes(&pa, rec_k) == cudaSuccess) a.direct = pa.type == cudaMemoryTypeHost;
   else (void)cudaGetLastError();
-  const int cols = (a.rep < 8 ? a.rep : 8) * L;
+  // Heads of a CTA: as many as fill 8 columns with their rows.  More heads mean a longer union that every tile
+  // of columns decodes anew, fewer leave columns empty: 64 rows of one sequence, 64 groups opened by each of 8
+  // heads, take 30 us with one head a CTA and 79 with 8 where the heads opened different groups (29 with 8
+  // where all opened the same), 2 rows of each of 16 sequences 44 with 4 and 59 with 8 (21 and 23).
+  a.hpc = L >= 8 ? 1 : 8 / L;
+  if (a.hpc > a.rep) a.hpc = a.rep;
+  // One row of few sequences: half as many heads where twice the CTAs are still resident (4 sequences 13.9
+  // against 17.4 us, or 11.1 and 11.2 with the same groups for all heads).
+  if (L == 1 && (int64_t)p.batch * p.kv_heads * ((a.rep + a.hpc - 1) / a.hpc) * 16 <= 132 * kv4::ctas_of(1))
+    a.hpc = (a.hpc + 1) / 2;
+  const int cols = a.hpc * L;
   const bool wide = cols > 8;
-  const int64_t ctas = (int64_t)p.batch * p.kv_heads * ((a.rep + 7) / 8) * ((cols + (wide ? 15 : 7)) / (wide ? 16 : 8));
+  const int64_t ctas = (int64_t)p.batch * p.kv_heads * ((a.rep + a.hpc - 1) / a.hpc) * ((cols + (wide ? 15 : 7)) / (wide ? 16 : 8));
   // CTAs per tile: as many as are resident at once, at most 8 (a portable cluster).  Clusters of 4 to 8 leave
   // about a tenth of the places empty (33 of 8 CTAs fit where 37 would): a 36th of 8 would wait for a second round.
   const int64_t room = 132 * kv4::ctas_of(wide ? 2 : 1);
