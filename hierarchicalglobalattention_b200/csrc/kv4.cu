@@ -1,11 +1,15 @@
 // 4-bit KV record: pack, unpack, and the portable attention over it (any type, head_dim a multiple of 64).
 // The record's format is in kv4_common.cuh.
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "fp32x2.cuh"
 #include "kv4_common.cuh"
 
 namespace hga {
+
+namespace cg = cooperative_groups;
 
 HGA_DEVICE_ERROR_WORD(g_kv4_error, kv4_error_status)
 
@@ -373,139 +377,296 @@ cudaError_t launch_kv4_unpack(int dtype, int dh, int64_t bk, int64_t rows, const
 }
 
 // ---- attention, portable ------------------------------------------------------------------------
-constexpr int kPortRows = 8;    // query rows per CTA, two per warp
 constexpr int kPortWarps = 4;
 
-// One CTA per (query head, sequence, 8 query rows); units of 16 keys pass through shared memory as fp32,
-// a lane pair scores one key, and every warp keeps its rows' online softmax in registers.
-template <typename T, int DH>
+// The rows of a CTA, its units in shared memory as fp32 (K and V, a warp's own), the rows' queries (afterwards the
+// CTA's result) and softmax states.
+template <int DH, int R> struct PortSmem {
+  static constexpr int LD = DH + 4;
+  static constexpr int kUnit = 2 * kKv4Unit * LD;             // floats of a warp
+  static constexpr int kRows = kPortWarps * kUnit;            // [R][DH]
+  static constexpr int kMax = kRows + R * DH, kSum = kMax + (kPortWarps + 1) * R;  // [warps, then the CTA][R]
+  static constexpr int kTotal = (kSum + (kPortWarps + 1) * R) * 4;
+};
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const T* t = reinterpret_cast<const T*>(&w);
+    return make_float4(Num<T>::to_f(t[0]), Num<T>::to_f(t[1]), Num<T>::to_f(t[2]), Num<T>::to_f(t[3]));
+  }
+}
+template <typename MT>
+__device__ __forceinline__ float2 scale_min(const uint8_t* meta, int pair) {
+  const uint32_t w = reinterpret_cast<const uint32_t*>(meta)[pair];
+  const MT* t = reinterpret_cast<const MT*>(&w);
+  return make_float2(Num<MT>::to_f(t[0]), Num<MT>::to_f(t[1]));
+}
+
+// Any type and head_dim, fp32 throughout.  A cluster serves up to R rows of one query head; the units of 16 keys
+// (slots and the head's own opened groups) are dealt to its warps, each of which decodes a unit into
+// shared memory, scores a key with a lane pair and keeps its own online softmax of all R rows in registers.
+// The partial results are joined as in the matrix kernel: warps, then CTAs, in a fixed order.
+// Bound by issue (decoding into fp32 and plain FMAs) and, for one sequence, by latency: one token of 32 heads
+// over 4 at 32768 in fp32 13.6 us, a block of 64 rows 262 us; with the units one after the other in one CTA per
+// head and bytes decoded one by one 409 and 835.
+template <typename T, int DH, int R>
 __global__ void __launch_bounds__(kPortWarps * 32) attend_kv4_kernel(
     hga_params p, int L, const T* __restrict__ q, const int32_t* __restrict__ seq_pos, const T* __restrict__ hot_k,
     const T* __restrict__ hot_v, int64_t hot_cap, const uint8_t* rec_k, const uint8_t* rec_v, int64_t unit_cap,
     const int32_t* __restrict__ open_gid, const int32_t* __restrict__ open_t0, int Kg, T* __restrict__ out) {
   using MT = typename Kv4Meta<T>::type;
-  constexpr int LD = DH + 2, VD = DH / 32;
-  __shared__ float qs[kPortRows][LD], ks[kKv4Unit][LD], vs[kKv4Unit][LD];
-  const int h = blockIdx.x, b = blockIdx.y, row0 = blockIdx.z * kPortRows;
-  const int H = p.nhead, KVH = p.kv_heads, C = p.chunk_size, gs = p.group_size, U = gs / kKv4Unit;
-  const int kvh = h / (H / KVH);
+  using S = PortSmem<DH, R>;
+  constexpr int LD = S::LD, VD = DH / 32;
+  extern __shared__ __align__(16) float port_smem[];
+  const int tiles = (L + R - 1) / R;
+  const int rank = blockIdx.x, splits = gridDim.x, h = blockIdx.y, b = blockIdx.z / tiles, row0 = blockIdx.z % tiles * R;
+  const int H = p.nhead, KVH = p.kv_heads, C = p.chunk_size, U = p.group_size / kKv4Unit;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int nrows = L - row0 < kPortRows ? L - row0 : kPortRows;
+  const int nrows = L - row0 < R ? L - row0 : R;
   const int pos = seq_pos[b];
   const int kf = p.keep_first > 0 ? p.keep_first : 0, kl = p.keep_last > 0 ? p.keep_last : 0;
-  const size_t bh = (size_t)b * H + h;
+  const size_t bh = (size_t)b * H + h, bk = (size_t)b * KVH + h / (H / KVH);
   T* o_base = out + (bh * L + row0) * DH;
   const int n_closed = pos / C, c0 = pos % C;
   if (pos < 0 || c0 + L > C || (int64_t)(kf + kl + 1) * C > hot_cap) {
     if (tid == 0) atomicCAS(&g_kv4_error, 0, kErrBoundsAttendKv4);
-    for (int i = tid; i < nrows * DH; i += blockDim.x) o_base[i] = Num<T>::from_f(0.f);
-    return;
+    if (rank == 0)
+      for (int i = tid; i < nrows * DH; i += blockDim.x) o_base[i] = Num<T>::from_f(0.f);
+    return;  // the whole cluster
+  }
+  float* qs = port_smem + S::kRows;
+  float* ks = port_smem + warp * S::kUnit;
+  float* vs = ks + kKv4Unit * LD;
+  for (int i = tid; i < R * DH; i += blockDim.x) qs[i] = i / DH < nrows ? Num<T>::to_f(q[(bh * L + row0) * DH + i]) : 0.f;
+  __syncthreads();
+  float o[R][VD], m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int d = 0; d < VD; ++d) o[r][d] = 0.f;
   }
   int f_hi, l_lo;
   windows(n_closed, kf, kl, f_hi, l_lo);
-  for (int i = tid; i < kPortRows * DH; i += blockDim.x)
-    qs[i / DH][i % DH] = i / DH < nrows ? Num<T>::to_f(q[(bh * L + row0) * DH + i]) : 0.f;
-  float o[2][VD], m[2], l[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < VD; ++d) o[i][d] = 0.f;
-  }
-  // one unit: from the slots (chunk >= 0) or the record (unit number), key j visible to row t iff
-  // t >= tmin + causal * j
-  auto take = [&](int64_t hot_row, int64_t unit, int tmin, int causal, int count) {
-    __syncthreads();
-    if (unit < 0) {
-      const size_t base = (((size_t)b * KVH + kvh) * hot_cap + hot_row) * DH;
-      for (int i = tid; i < kKv4Unit * DH; i += blockDim.x) {
-        const bool in = i / DH < count;  // rows past the block hold an earlier sequence's values
-        ks[i / DH][i % DH] = in ? Num<T>::to_f(hot_k[base + i]) : 0.f;
-        vs[i / DH][i % DH] = in ? Num<T>::to_f(hot_v[base + i]) : 0.f;
+  const int wu = C / kKv4Unit, n_first = f_hi * wu, n_win = n_first + (n_closed - l_lo) * wu;
+  const int nact = c0 + row0 + nrows, n_hot = n_win + (nact + kKv4Unit - 1) / kKv4Unit, n_all = n_hot + Kg * U;
+  for (int i = rank * kPortWarps + warp; i < n_all; i += splits * kPortWarps) {
+    // key j of the unit is visible to row t iff j < count and t >= tmin + causal * j
+    int tmin = 0, causal = 0, count = kKv4Unit;
+    __syncwarp();  // the last unit has been read
+    if (i < n_hot) {
+      int64_t row;
+      if (i < n_first) {
+        row = (int64_t)i * kKv4Unit;
+      } else if (i < n_win) {
+        row = (int64_t)(kf + (l_lo + (i - n_first) / wu) % (kl > 0 ? kl : 1)) * C + (i - n_first) % wu * kKv4Unit;
+      } else {
+        const int act = (i - n_win) * kKv4Unit;
+        row = (int64_t)(kf + kl) * C + act;
+        tmin = act - c0;
+        causal = 1;
+        if (nact - act < count) count = nact - act;
+      }
+      const size_t base = (bk * hot_cap + row) * DH;
+#pragma unroll 4
+      for (int x = lane; x < kKv4Unit * DH / 4; x += 32) {
+        const int tok = x / (DH / 4), c4 = x % (DH / 4) * 4;
+        const bool in = tok < count;  // rows past the block hold an earlier sequence's values
+        *reinterpret_cast<float4*>(ks + tok * LD + c4) = in ? load4<T>(hot_k + base + x * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(vs + tok * LD + c4) = in ? load4<T>(hot_v + base + x * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     } else {
-      const size_t base = (((size_t)b * KVH + kvh) * unit_cap + unit) * kv4_unit_bytes(DH);
-      for (int i = tid; i < 2 * kKv4Unit * DH; i += blockDim.x) {
-        const bool is_v = i >= kKv4Unit * DH;
-        const int x = is_v ? i - kKv4Unit * DH : i, tok = x / DH, ch = x % DH;
-        const uint8_t* u = (is_v ? rec_v : rec_k) + base;
-        const int r = is_v ? ch & 15 : tok, c = is_v ? tok : ch & 15, nib = kv4_nibble(r, c);
-        const uint32_t n = (u[kv4_word_byte(ch >> 4, r, c) + nib / 2] >> (4 * (nib & 1))) & 15u;
-        const MT* pair = reinterpret_cast<const MT*>(u + 8 * DH) + 2 * (tok * (DH / 32) + ch / 32);
-        const float y = fmaf((float)n, Num<MT>::to_f(pair[0]), Num<MT>::to_f(pair[1]));
-        if (is_v) vs[tok][ch] = y; else ks[tok][ch] = y;
+      const int j = (i - n_hot) / U, gid = open_gid[bh * Kg + j];
+      tmin = open_t0[bh * Kg + j];
+      if (gid < 0 || tmin < 0 || tmin >= row0 + nrows) continue;
+      if (((int64_t)gid + 1) * U > unit_cap) {
+        if (lane == 0) atomicCAS(&g_kv4_error, 0, kErrBoundsAttendKv4);
+        continue;
+      }
+      const size_t base = (bk * unit_cap + (int64_t)gid * U + (i - n_hot) % U) * kv4_unit_bytes(DH);
+      // a lane's words hold rows g, g + 8 and columns 2c, 2c + 1, 2c + 8, 2c + 9 of their tiles
+      const int g = lane >> 2, c = 2 * (lane & 3);
+      const uint8_t *uk = rec_k + base, *uv = rec_v + base;
+#pragma unroll
+      for (int quad = 0; quad < DH / 64; ++quad) {
+        const uint4 k4 = *reinterpret_cast<const uint4*>(uk + (quad * 32 + lane) * 16);
+        const uint4 v4 = *reinterpret_cast<const uint4*>(uv + (quad * 32 + lane) * 16);
+        const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w}, vw[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+          const int blk = quad * 2 + t2;  // 32 channels: two tiles
+          float2 km[2], vm[4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) km[r] = scale_min<MT>(uk + 8 * DH, (g + 8 * r) * VD + blk);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vm[e] = scale_min<MT>(uv + 8 * DH, (c + (e & 1) + 8 * (e >> 1)) * VD + blk);
+#pragma unroll
+          for (int t1 = 0; t1 < 2; ++t1) {
+            const int ch = blk * 32 + t1 * 16;
+            const uint32_t wk = kw[t2 * 2 + t1], wv = vw[t2 * 2 + t1];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {  // row half n & 1, column half n >> 1; the pair's second column 4 nibbles on
+              const int r = n & 1, e = n >> 1;
+              *reinterpret_cast<float2*>(ks + (g + 8 * r) * LD + ch + c + 8 * e) =
+                  make_float2(fmaf((float)(wk >> (4 * n) & 15u), km[r].x, km[r].y),
+                              fmaf((float)(wk >> (4 * n + 16) & 15u), km[r].x, km[r].y));
+              vs[(c + 8 * e) * LD + ch + g + 8 * r] = fmaf((float)(wv >> (4 * n) & 15u), vm[2 * e].x, vm[2 * e].y);
+              vs[(c + 1 + 8 * e) * LD + ch + g + 8 * r] = fmaf((float)(wv >> (4 * n + 16) & 15u), vm[2 * e + 1].x, vm[2 * e + 1].y);
+            }
+          }
+        }
       }
     }
-    __syncthreads();
-    const int key = lane >> 1, half = lane & 1;
+    __syncwarp();
+    const int key = lane >> 1, half = 2 * (lane & 1);
+    float dot[R];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = warp * 2 + i, t = row0 + r;
-      if (r >= nrows) continue;  // warp-uniform
-      float dot = 0.f;
-      for (int d = half; d < DH; d += 2) dot = fmaf(qs[r][d], ks[key][d], dot);
-      dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-      const bool vis = key < count && t >= tmin + causal * key;
+    for (int r = 0; r < R; ++r) dot[r] = 0.f;
+#pragma unroll 8
+    for (int d = half; d < DH; d += 4) {
+      const float2 kv = *reinterpret_cast<const float2*>(ks + key * LD + d);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float2 qv = *reinterpret_cast<const float2*>(qs + r * DH + d);
+        dot[r] = fmaf(qv.y, kv.y, fmaf(qv.x, kv.x, dot[r]));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r >= nrows) break;
+      const float x = dot[r] + __shfl_xor_sync(0xffffffffu, dot[r], 1);
+      const bool vis = key < count && row0 + r >= tmin + causal * key;
       const unsigned mask = __ballot_sync(0xffffffffu, vis);
       if (!mask) continue;
-      const float s = vis ? dot * p.scale * 1.4426950408889634f : -INFINITY;
+      const float s = vis ? x * p.scale * 1.4426950408889634f : -INFINITY;
       float mx = s;
 #pragma unroll
       for (int w = 16; w >= 2; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-      const float m_new = fmaxf(m[i], mx);
+      const float m_new = fmaxf(m[r], mx);
       const float base = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2f(m[i] - base), pe = vis ? exp2f(s - base) : 0.f;
-      float ps = half ? 0.f : pe;
+      const float alpha = exp2f(m[r] - base), pe = vis ? exp2f(s - base) : 0.f;
+      float ps = pe;
 #pragma unroll
-      for (int w = 16; w; w >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, w);
-      l[i] = l[i] * alpha + ps;
-      m[i] = m_new;
+      for (int w = 16; w >= 2; w >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, w);
+      l[r] = l[r] * alpha + ps;
+      m[r] = m_new;
 #pragma unroll
-      for (int d = 0; d < VD; ++d) o[i][d] *= alpha;
+      for (int d = 0; d < VD; ++d) o[r][d] *= alpha;
+#pragma unroll
       for (int j = 0; j < kKv4Unit; ++j) {
         const float pj = __shfl_sync(0xffffffffu, pe, 2 * j);
         if (!(mask >> (2 * j) & 1)) continue;  // what an invisible key holds does not count, NaN included
 #pragma unroll
-        for (int d = 0; d < VD; ++d) o[i][d] = fmaf(pj, vs[j][lane + 32 * d], o[i][d]);
+        for (int d = 0; d < VD; ++d) o[r][d] = fmaf(pj, vs[j * LD + lane + 32 * d], o[r][d]);
       }
     }
-  };
-  const int wu = C / kKv4Unit;
-  for (int u = 0; u < f_hi * wu; ++u) take((int64_t)u * kKv4Unit, -1, 0, 0, kKv4Unit);
-  for (int n = l_lo; n < n_closed; ++n)
-    for (int u = 0; u < wu; ++u) take((int64_t)(kf + n % (kl > 0 ? kl : 1)) * C + u * kKv4Unit, -1, 0, 0, kKv4Unit);
-  for (int j = 0; j < Kg; ++j) {
-    const int gid = open_gid[bh * Kg + j], t0 = open_t0[bh * Kg + j];
-    if (gid < 0 || t0 < 0) continue;
-    if (((int64_t)gid + 1) * U > unit_cap) {
-      if (tid == 0) atomicCAS(&g_kv4_error, 0, kErrBoundsAttendKv4);
-      continue;
+  }
+  __syncthreads();
+  float *pm = port_smem + S::kMax, *pl = port_smem + S::kSum;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int d = 0; d < VD; ++d) ks[r * DH + lane + 32 * d] = o[r][d];
+    if (lane == 0) {
+      pm[warp * R + r] = m[r];
+      pl[warp * R + r] = l[r];
     }
-    for (int u = 0; u < U; ++u) take(0, (int64_t)gid * U + u, t0, 0, kKv4Unit);
   }
-  const int nact = c0 + row0 + nrows;
-  for (int u = 0; u * kKv4Unit < nact; ++u)
-    take((int64_t)(kf + kl) * C + u * kKv4Unit, -1, u * kKv4Unit - c0, 1,
-         nact - u * kKv4Unit < kKv4Unit ? nact - u * kKv4Unit : kKv4Unit);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = warp * 2 + i;
-    if (r >= nrows) continue;
-#pragma unroll
-    for (int d = 0; d < VD; ++d) o_base[(size_t)r * DH + lane + 32 * d] = Num<T>::from_f(o[i][d] / l[i]);
+  __syncthreads();
+  if (tid < R) {
+    float mx = -INFINITY, sum = 0.f;
+    for (int w = 0; w < kPortWarps; ++w) mx = fmaxf(mx, pm[w * R + tid]);
+    for (int w = 0; w < kPortWarps; ++w) {
+      // a maximum of -infinity: nothing seen (sum 0), or only scores that are NaN (sum NaN)
+      const float mw = pm[w * R + tid], lw = pl[w * R + tid], f = mw == -INFINITY ? lw : exp2f(mw - mx);
+      sum += f * lw;
+      pm[w * R + tid] = f;
+    }
+    pm[kPortWarps * R + tid] = mx;
+    pl[kPortWarps * R + tid] = sum;
   }
+  __syncthreads();
+  for (int i = tid; i < nrows * DH; i += blockDim.x) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPortWarps; ++w) {
+      const float f = pm[w * R + i / DH];
+      s += f == 0.f ? 0.f : f * port_smem[w * S::kUnit + i];
+    }
+    qs[i] = s;
+  }
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  const int lo = DH * rank / splits, width = DH * (rank + 1) / splits - lo;
+  for (int i = tid; i < width * nrows; i += blockDim.x) {
+    const int r = i / width, ch = lo + i % width;
+    float mr[8], lr[8], vr[8], mx = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k >= splits) break;
+      const float* other = cl.map_shared_rank(port_smem, k);
+      mr[k] = other[S::kMax + kPortWarps * R + r];
+      lr[k] = other[S::kSum + kPortWarps * R + r];
+      vr[k] = other[S::kRows + r * DH + ch];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < splits) mx = fmaxf(mx, mr[k]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k >= splits) break;
+      const float f = mr[k] == -INFINITY ? lr[k] : exp2f(mr[k] - mx);
+      if (f == 0.f) continue;
+      sum += f * lr[k];
+      acc += f * vr[k];
+    }
+    o_base[(size_t)r * DH + ch] = Num<T>::from_f(acc / sum);
+  }
+  cl.sync();  // no CTA leaves while another still reads its result
+}
+
+template <typename T, int DH, int R>
+static cudaError_t port_t(const hga_params& p, int L, const void* q, const int32_t* seq_pos, const void* hk,
+                          const void* hv, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
+                          const int32_t* og, const int32_t* ot, int Kg, void* out, cudaStream_t st) {
+  constexpr int smem = PortSmem<DH, R>::kTotal;
+  auto kern = attend_kv4_kernel<T, DH, R>;
+  static unsigned long long raised = 0;
+  cudaError_t e = raise_smem_limit((const void*)kern, smem, &raised);
+  if (e != cudaSuccess) return e;
+  // CTAs along the units: as many as are resident, at most 8 (clusters leave about a tenth of the places empty)
+  const int64_t ctas = (int64_t)p.nhead * p.batch * ((L + R - 1) / R);
+  int64_t splits = 132 * (200 * 1024 / smem < 4 ? 200 * 1024 / smem : 4) / ctas;
+  splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)splits, p.nhead, (unsigned)((int64_t)p.batch * ((L + R - 1) / R)));
+  cfg.blockDim = dim3(kPortWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p, L, (const T*)q, seq_pos, (const T*)hk, (const T*)hv, hot_cap,
+                            (const uint8_t*)rec_k, (const uint8_t*)rec_v, unit_cap, og, ot, Kg, (T*)out);
 }
 
 cudaError_t launch_attend_kv4(const hga_params& p, int L, const void* q, const int32_t* seq_pos, const void* hk,
                               const void* hv, int64_t hot_cap, const void* rec_k, const void* rec_v, int64_t unit_cap,
                               const int32_t* og, const int32_t* ot, int Kg, void* out, cudaStream_t st) {
   const int dtype = p.dtype, dh = p.head_dim;
-  const dim3 grid(p.nhead, p.batch, (L + kPortRows - 1) / kPortRows);
-  HGA_KV4_DISPATCH((attend_kv4_kernel<T, DH><<<grid, kPortWarps * 32, 0, st>>>(
-      p, L, (const T*)q, seq_pos, (const T*)hk, (const T*)hv, hot_cap, (const uint8_t*)rec_k, (const uint8_t*)rec_v,
-      unit_cap, og, ot, Kg, (T*)out)))
-  return cudaGetLastError();
+#define HGA_KV4_PORT(RR) port_t<T, DH, RR>(p, L, q, seq_pos, hk, hv, hot_cap, rec_k, rec_v, unit_cap, og, ot, Kg, out, st)
+  cudaError_t e = cudaSuccess;
+  HGA_KV4_DISPATCH((e = L == 1 ? HGA_KV4_PORT(1) : HGA_KV4_PORT(8)))
+#undef HGA_KV4_PORT
+  return e;
 }
 
 }  // namespace hga

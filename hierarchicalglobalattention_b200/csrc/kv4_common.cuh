@@ -29,10 +29,4 @@ template <> struct Kv4Meta<float> { using type = __nv_bfloat16; };
 
 __host__ __device__ constexpr int kv4_unit_bytes(int dh) { return 10 * dh; }
 
-// Byte of the tile words and nibble that hold (row r, column c) of tile t.
-__device__ __forceinline__ int kv4_word_byte(int t, int r, int c) {
-  return ((t >> 2) * 128 + (4 * (r & 7) + ((c & 7) >> 1)) * 4 + (t & 3)) * 4;
-}
-__device__ __forceinline__ int kv4_nibble(int r, int c) { return (r >> 3) + 2 * (c >> 3) + 4 * (c & 1); }
-
 }  // namespace hga
