@@ -51,9 +51,10 @@ def q_view(q: torch.Tensor) -> Tuple[torch.Tensor, int]:
 def kv_cap_of(t: torch.Tensor) -> int:
     """Rows allocated per (batch, kv-head) of a [B,KVH,S,Dh] view into a [B,KVH,cap,Dh] buffer."""
     B, KVH, S, Dh = t.shape
-    if t.stride(3) != 1 or t.stride(2) != Dh or t.stride(1) % Dh or t.stride(0) != KVH * t.stride(1):
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or s2 != Dh or s1 % Dh or s0 != KVH * s1:
         raise _lib.HgaError(f"K/V tensor must be a row-slice of a contiguous [B,KVH,cap,Dh] buffer; strides {t.stride()}")
-    return t.stride(1) // Dh
+    return s1 // Dh
 
 
 def summaries(p: HgaParams, k_raw: torch.Tensor, k_rope: torch.Tensor, v: torch.Tensor,
@@ -409,7 +410,7 @@ def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     r = x if len(shape) == 2 and x.is_contiguous() else _rows(x)
     dev = x.device
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
-    scale = x.new_empty((*shape[:-1], -(-K // FP8_BLOCK)), dtype=torch.float32)
+    scale = torch.empty(*shape[:-1], -(-K // FP8_BLOCK), device=dev, dtype=torch.float32)
     rc = lib().hga_fp8_quantize(r.shape[0], K, code, r.data_ptr(), max(r.stride(0), K), q.data_ptr(), K,
                                 scale.data_ptr(), stream_ptr(dev))
     if rc:
@@ -478,7 +479,7 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     r = x if len(shape) == 2 and x.is_contiguous() else _rows(x)
     M = r.shape[0]
     if out is None:
-        out = x.new_empty((*shape[:-1], N), dtype=out_dtype)
+        out = torch.empty(*shape[:-1], N, device=dev, dtype=out_dtype)
     elif out.dtype != out_dtype or out.shape != (*shape[:-1], N) or not out.is_contiguous():
         raise _lib.HgaError("fp8_linear: out must be a contiguous [..., N] tensor of the result's type")
     h = lib()
@@ -559,7 +560,7 @@ def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor,
     units = -(-S // KV4_UNIT)
     if rec is None:
         cap = unit0 + units
-        rec_k = k.new_empty((B, KVH, cap, 10 * Dh), dtype=torch.uint8)
+        rec_k = torch.empty(B, KVH, cap, 10 * Dh, device=k.device, dtype=torch.uint8)
         rec_v = torch.empty_like(rec_k)
     else:
         rec_k, rec_v = rec
