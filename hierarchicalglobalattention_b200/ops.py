@@ -627,6 +627,8 @@ def attend_decode_kv4(p: HgaParams, q: torch.Tensor, seq_pos: torch.Tensor, hot_
     if (hot_k.dtype != dtype or hot_v.dtype != dtype or hot != hot_v.shape or len(hot) != 4 or hot[0] != B
             or hot[1] != KVH or hot[3] != Dh or hot_k.stride() != hot_v.stride()):
         raise _lib.HgaError("attend_decode_kv4: hot_k / hot_v must have q's type, [B,KVH,rows,Dh] and one layout")
+    if hot[2] < (max(p.keep_first, 0) + max(p.keep_last, 0) + 1) * p.chunk_size:
+        raise _lib.HgaError("attend_decode_kv4: hot_k / hot_v need slots for keep_first + keep_last + 1 chunks")
     i32 = torch.int32
     if (seq_pos.dtype != i32 or open_gid.dtype != i32 or open_t0.dtype != i32 or seq_pos.numel() != B
             or open_gid.shape != open_t0.shape or open_gid.shape[:2] != (B, H)):

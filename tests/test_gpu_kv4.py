@@ -374,6 +374,8 @@ def test_refusals(cuda):
                 _run({**st, name: bad}, cuda)
             with pytest.raises(E, match="one layout"):
                 _run({**st, "hk": bad, "hv": bad}, cuda)
+    with pytest.raises(E, match="slots"):
+        _run({**st, "hk": st["hk"][:, :, 1:], "hv": st["hv"][:, :, 1:]}, cuda)
     dev = (st["q"].to(cuda), st["pos"].to(cuda), st["hk"].to(cuda), st["hv"].to(cuda), *st["rec"], st["gid"].to(cuda),
            st["t0"].to(cuda))
     with pytest.raises(E, match="out must be"):
