@@ -18,9 +18,9 @@
 // cycles of about 1100, the rest is the epilogue's chain (barrier 290, two reads of 215, 64 paired FMAs and their
 // loop 400; two warps a scheduler, 128 sums a thread).  Measured and not kept: one CTA on 128 x 256 tiles
 // (48 KB of loads a block) 470 us, sixteen epilogue warps of 64 columns 370 (440 with scales ahead, which
-// spill; 395 with two more warps bringing the scales into shared memory), reads 32 columns ahead of the sums 400, 256 x 128 tiles in four TMEM buffers 570, a block's
-// two halves of 128 features as MMAs and hand-overs of their own 375, arrivals with cluster-scope release 690 (a
-// memory barrier each).
+// spill; 395 with two more warps bringing the scales into shared memory), reads 32 columns ahead of the sums
+// 400, 256 x 128 tiles in four TMEM buffers 570, a block's two halves of 128 features as MMAs and hand-overs of
+// their own 375, arrivals with cluster-scope release 690 (a memory barrier each).
 // Results go through two 4 KB pieces of swizzled shared memory per warp to whole-line TMA stores (plain stores where
 // the output's rows are off the 16-byte grid).  Waits are bounded as in tc_common.cuh.
 #include "fp8_common.cuh"
