@@ -13,14 +13,15 @@
 //   warp 1      MMA issuer (of the even CTA), TMEM owner
 //   warps 4-11  each reads 32 TMEM lanes (rows) x BN / 2 columns: one row a thread, one weight block a
 //               warp, so a block's scale is one product per thread
-// What bounds it: a block's products have to be handed over and added before their TMEM buffer can be used again.
-// 32768 x 2048 into 5120 features: 340 us, 2.0 PFLOP/s in a burst; the MMAs of a 256 x 256 x 128 block take 512
-// cycles of about 1100, the rest is the epilogue's chain (barrier 290, two reads of 215, 64 paired FMAs and their
-// loop 400; two warps a scheduler, 128 sums a thread).  Measured and not kept: one CTA on 128 x 256 tiles
-// (48 KB of loads a block) 470 us, sixteen epilogue warps of 64 columns 370 (440 with scales ahead, which
-// spill; 395 with two more warps bringing the scales into shared memory), reads 32 columns ahead of the sums
-// 400, 256 x 128 tiles in four TMEM buffers 570, a block's two halves of 128 features as MMAs and hand-overs of
-// their own 375, arrivals with cluster-scope release 690 (a memory barrier each).
+// What bounds it: the loop that a TMEM buffer turns in (MMAs, commit, epilogue, release, next MMAs; two buffers of
+// 256 columns are all of TMEM).  32768 x 2048 into 5120 features: 335 us, 2.05 PFLOP/s in a burst; the MMAs of a
+// 256 x 256 x 128 block take 512 cycles of about 1100.  With the epilogue's reads and sums left out the tiles still
+// took 290 us; three stages of loads instead of five, or every load from the same tile, changed nothing.
+// Measured and not kept: one CTA on 128 x 256 tiles (48 KB of loads a block) 470 us, sixteen epilogue warps of 64
+// columns 370 (440 with scales ahead, which spill; 395 with two more warps bringing the scales into shared
+// memory), reads 32 columns ahead of the sums 400, 256 x 128 tiles in four TMEM buffers 570, a block's two halves
+// of 128 features as MMAs and hand-overs of their own 375, arrivals with cluster-scope release 690 (a memory
+// barrier each).
 // Results go through two 4 KB pieces of swizzled shared memory per warp to whole-line TMA stores (plain stores where
 // the output's rows are off the 16-byte grid).  Waits are bounded as in tc_common.cuh.
 #include "fp8_common.cuh"
@@ -191,8 +192,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int tile = group; tile < a.tiles && ok; tile += groups) {
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
           const int buf = it & 1;
-          if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(d_empty + buf, (it / 2 - 1) & 1, abort_flag, kErrFp8 + 2));
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(full + st, phase, abort_flag, kErrFp8 + 1));
+          // the buffer's release comes last: it is what the loop turns on (with it first 379 against 374 us)
+          ok = __all_sync(0xffffffffu, mbar_wait(full + st, phase, abort_flag, kErrFp8 + 1));
+          if (it >= 2) ok = ok && __all_sync(0xffffffffu, mbar_wait(d_empty + buf, (it / 2 - 1) & 1, abort_flag, kErrFp8 + 2));
           if (!ok) break;
           fence_after();
           const uint64_t dx = dx0 + (uint64_t)(st * (S::kStage >> 4)), dw = dw0 + (uint64_t)(st * (S::kStage >> 4));
