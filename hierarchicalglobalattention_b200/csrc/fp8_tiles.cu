@@ -75,7 +75,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+// until the sources of all but the latest N stores of this thread have been read
+template <int N> __device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // One lane of the warp, the same one every time; all lanes call.
@@ -280,7 +283,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (n0 + c >= a.n || m0 >= a.m) break;  // warp-uniform
         unsigned char* stg = stage + ((c / PC) & 1) * 4096;
         if (PAIR == 2 || a.tma_out) {
-          if (lane == 0) bulk_wait_read1();  // the store before the last has been read out
+          // The store that used this piece before has been read out.  Within a tile that is the store before
+          // the last; a tile begins with piece 0 whichever the last tile ended with (one pass of 16-bit results in a
+          // 64-column part, an odd number at a ragged edge), so its first pass waits for every store.
+          if (lane == 0) {
+            if (c == 0) bulk_wait_read<0>(); else bulk_wait_read<1>();
+          }
           __syncwarp();
         }
 #pragma unroll
