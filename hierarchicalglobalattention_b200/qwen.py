@@ -40,6 +40,7 @@ from .fp8 import fp8_concat
 from .module import routed_attention
 from .router import ChunkRouter
 from .store import VramKVCacheStore
+from .weights import WeightSources
 
 
 def rope_theta_of(config: Any, default: float = 1_000_000.0) -> float:
@@ -163,17 +164,21 @@ class QwenRoutedAttention(nn.Module):
         quantised once (again when a weight changes)."""
         ts = tuple(m.weight for m in mods) + tuple(getattr(m, "weight_scale_inv", None) for m in mods) + tuple(
             getattr(m, "bias", None) for m in mods)
-        key = tuple((t.data_ptr(), t._version, t.dtype) if t is not None else None for t in ts)
         hit = self._fp8_cache.get(name)
-        if hit is None or hit[0] != key:
+        if hit is None or not hit[0].same(ts):
             whole = fp8_concat(mods)
             parts = [whole] if whole is not None else [fp8_concat([m]) for m in mods]
             if any(p is None for p in parts):
                 raise TypeError("fp8_projections needs nn.Linear layers or 8-bit layers with 128 x 128 block scales")
-            hit = (key, parts)
+            hit = (WeightSources(ts), parts)
             self._fp8_cache[name] = hit
         ys = [ops.fp8_linear(x, w, s, bias=None if b is None else b.to(x.dtype)) for w, s, b in hit[1]]
         return ys[0] if len(ys) == 1 else torch.cat(ys, dim=-1)
+
+    def refresh_weights(self) -> None:
+        """Make the quantised copies of the projections' weights again at the next call (needed only after
+        writes through ``.data``, which the tensors' version counters do not see)."""
+        self._fp8_cache.clear()
 
     def _o_proj(self, heads: torch.Tensor) -> torch.Tensor:
         return self._fp8(heads, "o", (self.orig.o_proj,)) if self.fp8_projections else self.orig.o_proj(heads)
