@@ -23,6 +23,7 @@ from . import ops
 from .config import ChunkPlacementPolicy, RouterConfig
 from .router import ChunkRouter
 from .store import VramKVCacheStore
+from .weights import WeightSources
 
 
 def routed_attention(router: ChunkRouter, layer: int, hp, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -120,15 +121,19 @@ class HierarchicalGlobalAttentionRouted(nn.Module):
         """Concatenated [q;k;v] projection weight (and bias), rebuilt when any parameter changes."""
         ps = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight,
               self.q_proj.bias, self.k_proj.bias, self.v_proj.bias)
-        key = tuple((p.data_ptr(), p._version, p.dtype) if p is not None else None for p in ps)
-        if self._qkv_cache is None or self._qkv_cache[0] != key:
+        if self._qkv_cache is None or not self._qkv_cache[0].same(ps):
             w = torch.cat([self.q_proj.weight, self.k_proj.weight, self.v_proj.weight], dim=0).detach()
             b = None
             if any(p is not None for p in ps[3:]):
                 b = torch.cat([p if p is not None else torch.zeros(q.weight.shape[0], device=w.device, dtype=w.dtype)
                                for p, q in zip(ps[3:], (self.q_proj, self.k_proj, self.v_proj))]).detach()
-            self._qkv_cache = (key, w, b)
+            self._qkv_cache = (WeightSources(ps), w, b)
         return self._qkv_cache[1], self._qkv_cache[2]
+
+    def refresh_weights(self) -> None:
+        """Make the concatenated projection weight again at the next call (needed only after writes through
+        ``.data``, which the parameters' version counters do not see)."""
+        self._qkv_cache = None
 
     def _own_rotary(self, n: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
         """fp32 cos/sin [n, Dh] (HierarchicalGlobalAttentionRouted.py:209-217), cached."""

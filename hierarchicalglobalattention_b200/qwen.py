@@ -147,14 +147,13 @@ class QwenRoutedAttention(nn.Module):
             return self._fp8(x, "qkv", projs)
         if all(type(m) is nn.Linear for m in projs):
             ps = tuple(m.weight for m in projs) + tuple(m.bias for m in projs)
-            key = tuple((t.data_ptr(), t._version, t.dtype) if t is not None else None for t in ps)
-            if self._qkv_cache is None or self._qkv_cache[0] != key:
+            if self._qkv_cache is None or not self._qkv_cache[0].same(ps):
                 w = torch.cat([m.weight for m in projs], dim=0).detach()
                 b = None
                 if any(m.bias is not None for m in projs):
                     b = torch.cat([m.bias if m.bias is not None else
                                    torch.zeros(m.out_features, device=w.device, dtype=w.dtype) for m in projs]).detach()
-                self._qkv_cache = (key, w, b)
+                self._qkv_cache = (WeightSources(ps), w, b)
             return F.linear(x, self._qkv_cache[1], self._qkv_cache[2])
         return torch.cat([m(x) for m in projs], dim=-1).contiguous()
 
@@ -176,8 +175,9 @@ class QwenRoutedAttention(nn.Module):
         return ys[0] if len(ys) == 1 else torch.cat(ys, dim=-1)
 
     def refresh_weights(self) -> None:
-        """Make the quantised copies of the projections' weights again at the next call (needed only after
-        writes through ``.data``, which the tensors' version counters do not see)."""
+        """Make the concatenated or quantised copies of the projections' weights again at the next call (needed
+        only after writes through ``.data``, which the tensors' version counters do not see)."""
+        self._qkv_cache = None
         self._fp8_cache.clear()
 
     def _o_proj(self, heads: torch.Tensor) -> torch.Tensor:

@@ -95,6 +95,27 @@ def test_unchanged_sources_are_derived_once_and_data_writes_after_refresh_8bit(p
     assert (w._qkv(x)[:, 128:192] == 4 * IN).all()
 
 
+def test_a_replaced_projection_at_the_same_address_is_seen_16bit():
+    w, orig, buf = _wrapper()
+    x = torch.ones(1, IN)
+    mod = hga.HierarchicalGlobalAttentionRouted(d_model=IN, nhead=2, kv_heads=1, head_dim=64)
+    mod.v_proj = _linear(buf["v"])
+    assert (w._qkv(x) == IN).all() and (mod._fused_qkv()[0][192:] == 1).all()
+    buf["v"][:] = 2.0                      # a fresh layer in the old one's memory
+    for m in (orig, mod):
+        at = m.v_proj.weight.data_ptr()
+        del m.v_proj
+        gc.collect()
+        m.v_proj = _linear(buf["v"])
+        assert m.v_proj.weight.data_ptr() == at and m.v_proj.weight._version == 0
+    assert (w._qkv(x)[:, 192:] == 2 * IN).all() and (mod._fused_qkv()[0][192:] == 2).all()
+    one = mod._fused_qkv()[0]
+    assert mod._fused_qkv()[0] is one      # unchanged sources: nothing is made again
+    mod.v_proj.weight.data.fill_(5.0)      # not counted
+    mod.refresh_weights()
+    assert (mod._fused_qkv()[0][192:] == 5).all()
+
+
 def test_sources_are_not_kept_alive_and_survive_copies():
     t = torch.ones(4, 4)
     s = WeightSources((t, None))
