@@ -621,8 +621,8 @@ __global__ void __launch_bounds__(kPortWarps * 32) attend_kv4_kernel(
     for (int k = 0; k < 8; ++k) {
       if (k >= splits) break;
       const float f = mr[k] == -INFINITY ? lr[k] : exp2f(mr[k] - mx);
+      sum += f * lr[k];  // with a factor of 0 too: a sum that is NaN is not lost
       if (f == 0.f) continue;
-      sum += f * lr[k];
       acc += f * vr[k];
     }
     o_base[(size_t)r * DH + ch] = Num<T>::from_f(acc / sum);

@@ -775,8 +775,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
     for (int r = 0; r < 8; ++r) {
       if (r >= a.splits) break;
       const float f = mr[r] == -INFINITY ? lr[r] : ex2(mr[r] - mx);
+      sum += f * lr[r];  // with a factor of 0 too: a sum that is NaN is not lost
       if (f == 0.f) continue;
-      sum += f * lr[r];
       acc += f * vr[r];
     }
     const int x = x0 + col;
