@@ -74,6 +74,12 @@ template <> struct Half2<__nv_bfloat16> {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
   }
+  static __device__ __forceinline__ uint32_t pack_down(float a, float b) {  // towards zero
+    uint32_t r;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+  }
+  static constexpr float kTiny = 1.17549435e-38f;  // 2^-126, the smallest normal
   static constexpr uint32_t kInf = 0x7f80u;
 };
 template <> struct Half2<__half> {
@@ -86,6 +92,12 @@ template <> struct Half2<__half> {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
   }
+  static __device__ __forceinline__ uint32_t pack_down(float a, float b) {  // towards zero
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+  }
+  static constexpr float kTiny = 5.9604645e-8f;  // 2^-24, the smallest subnormal
   static constexpr uint32_t kInf = 0x7c00u;
 };
 using BF = Half2<__nv_bfloat16>;
@@ -505,12 +517,20 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
       }
     }
     soften(s, vis);
-    uint32_t pb[NT][2];
+    // The weights as two 16-bit terms: these rows are exact, and one term alone would keep 8 significant bits
+    // (bf16) of every weight.  The first is rounded towards zero and the second is kept above zero, so that
+    // a value of infinity meets two positive factors (infinity - infinity is not what it stands for).  With one term
+    // the 64-row block took 30.0 us instead of 30.7, 16 sequences of 32768 26.2 instead of 26.4.
+    uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      pb[nt][0] = transpose8(H::pack(s[nt][0], s[nt][1]));
-      pb[nt][1] = transpose8(H::pack(s[nt][2], s[nt][3]));
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float s0 = s[nt][2 * r], s1 = s[nt][2 * r + 1];
+        const uint32_t w = H::pack_down(s0, s1);
+        pl[nt][r] = transpose8(H::pack(fmaxf(s0 - H::lo(w), fminf(s0, H::kTiny)), fmaxf(s1 - H::hi(w), fminf(s1, H::kTiny))));
+        pb[nt][r] = transpose8(w);
+      }
     // V^T: tokens 0-7 (lanes 0-15) and 8-15, channels 0-7 and 8-15 of each 16
     const int vr = (lane & 7) + ((lane >> 4) << 3);
     bool odd = false;
@@ -522,15 +542,9 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
       }
       odd = __any_sync(0xffffffffu, odd);
     }
-    if (!odd) {
-#pragma unroll
-      for (int mt = 0; mt < KS; ++mt) {
-        uint32_t f[4];
-        ldmatrix4<true>(f, vb + vr * DH * 2 + (((mt * 2 + (lane >> 3 & 1)) ^ (vr & 7)) << 4));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma<T>(o[mt][nt], f, pb[nt][0], pb[nt][1]);
-      }
-    } else {
+    if (odd) {
+      // such values by plain sums for the columns that see their rows, then zeros in their place: a product of 0
+      // either way for the other columns, whose bits do not change
       float* w = reinterpret_cast<float*>(smem + LY::kScratch) + warp * 16 * COLS;  // [16 keys][COLS], -1 = unseen
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -546,12 +560,30 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
             const int ch = mt * 16 + g + 8 * (e >> 1);
             const float v = Num<T>::to_f(*reinterpret_cast<const T*>(buf + 16 * DH * 2 + key * DH * 2 +
                                                                       (((ch >> 3) ^ (key & 7)) << 4) + (ch & 7) * 2));
+            if (fabsf(v) < INFINITY) continue;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const float x = w[key * COLS + nt * 8 + 2 * c + (e & 1)];
-              if (!(x < 0.f)) o[mt][nt][e] = fmaf(Num<T>::round(x), v, o[mt][nt][e]);
+              if (!(x < 0.f)) o[mt][nt][e] = fmaf(x, v, o[mt][nt][e]);
             }
           }
+      __syncwarp();
+      for (int j = lane; j < 16 * DH / 2; j += 32) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(buf + 16 * DH * 2) + j;
+        const uint32_t v = *at;
+        *at = ((v & H::kInf) == H::kInf ? 0u : v & 0xffffu) | ((v >> 16 & H::kInf) == H::kInf ? 0u : v & 0xffff0000u);
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt) {
+      uint32_t f[4];
+      ldmatrix4<true>(f, vb + vr * DH * 2 + (((mt * 2 + (lane >> 3 & 1)) ^ (vr & 7)) << 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma<T>(o[mt][nt], f, pb[nt][0], pb[nt][1]);
+        mma<T>(o[mt][nt], f, pl[nt][0], pl[nt][1]);
+      }
     }
     __syncwarp();
     if (i + stride < n_hot) issue_hot(i + stride);
