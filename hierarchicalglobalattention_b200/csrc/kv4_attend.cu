@@ -10,21 +10,22 @@
 // The record's codes are used as integers.  With n the code, (word >> 4 i) & 0x000f000f | magic is a register
 // of two values 128 + n (bf16; 1024 + n in fp16), and one packed subtraction makes them n - 8, exactly:
 //   q . k = sum_blocks  scale_b (sum q (n - 8)) + mid_b sum_b q,     mid_b = min_b + 8 scale_b
-//   o     = sum_keys    w (n - 8) + p mid_b,                         w = bf16(p scale_b)
-// so keys enter the scores unrounded, and a weight's product with the block's scale is rounded to bf16 once
-// (as the weights of any 16-bit attention are; fp16 results carry three more bits, so there w is two bf16
-// terms, and fp16 itself would lose small scales to its range).  The mid terms are fp32 sums beside the
-// products.  bf16 scores leave the 128 in the products and take 128 sum q off instead; with fp16's 1024 that cost
-// up to 1 % of a score (the instruction truncates its sums relative to their largest term), and in the
+//   o     = sum_keys    w (n - 8) + p mid_b,                         w = p scale_b
+// so keys enter the scores unrounded.  A weight's product with its block's scale is two bf16 terms, 16 bits together
+// (fp16 would lose small scales to its range), as are the weights of the exact rows in the cache's type: with one
+// bf16 term the results of bf16 caches were up to 38 % further from 64 bits than fp32 arithmetic's, at 26.4 us
+// against 28.0 for 16 sequences of 32768 and 30.7 against 32.4 for a block of 64 rows.  The mid terms are fp32 sums
+// beside the products.  bf16 scores leave the 128 in the products and take 128 sum q off instead; with fp16's 1024
+// that cost up to 1 % of a score (the instruction truncates its sums relative to their largest term), and in the
 // output, whose sum runs over all keys, a bf16 ulp.
 //
 // Units are dealt to the warps of the `splits` CTAs of a cluster (windows and the active chunk first,
 // then the union); every warp keeps its own online softmax and copies its next units with cp.async (plain
 // loads for records in pinned host memory, where asynchronous copies are slower).  Warps join in shared
 // memory, CTAs through distributed shared memory, in a fixed order: no atomics on results, one launch.
-// One token for each of 16 sequences of 32768 (32 heads over 4): 26 us for 63 MB (2.4 TB/s); issue of the
+// One token for each of 16 sequences of 32768 (32 heads over 4): 28 us for 63 MB (2.25 TB/s); issue of the
 // decoding bounds it there (some 400 instructions a unit and warp, 39 % of the SMs' issue), set-up and the two
-// cluster barriers (9 us together) for one sequence: 10.4 us at 4096 tokens.  One pass over keys per query head
+// cluster barriers (9 us together) for one sequence: 10.6 us at 4096 tokens.  One pass over keys per query head
 // with plain FMAs took 566 and 398 us.
 #include <cooperative_groups.h>
 
@@ -187,7 +188,6 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
   // 128 sum q is taken off in fp32 with an error of 1e-5 of a score)
   constexpr bool FP16 = H::kInf != 0x7f80u;
   constexpr float kOffK = FP16 ? 8.f : -128.f;
-  constexpr bool SPLIT = H::kInf != 0x7f80u;  // fp16: the weights of the record as two bf16 terms
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int rank = blockIdx.x, bk = blockIdx.y, b = bk / p.kv_heads, kvh = bk % p.kv_heads;
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
         for (int k = 0; k < 2; ++k) {
           uint32_t f[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = SPLIT ? codes<H>(word[hb2 * 2 + k], e) : (word[hb2 * 2 + k] >> (4 * e) & 0x000f000fu) | H::kMagic;
+          for (int e = 0; e < 4; ++e) f[e] = FP16 ? codes<H>(word[hb2 * 2 + k], e) : (word[hb2 * 2 + k] >> (4 * e) & 0x000f000fu) | H::kMagic;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const uint2 v = qf[(nt * KS + blk * 2 + k) * 32 + lane];
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
 #pragma unroll
       for (int hb2 = 0; hb2 < 2; ++hb2) {
         const int blk = quad * 2 + hb2;
-        uint32_t wb[NT][2], wl[SPLIT ? NT : 1][2];
+        uint32_t wb[NT][2], wl[NT][2];  // weight x scale as two bf16 terms
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const uint32_t vm = *reinterpret_cast<const uint32_t*>(dv + 8 * DH + ((g + 8 * r) * NB + blk) * 4);
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
             corr[blk][nt][0] = d0;
             corr[blk][nt][1] = d1;
             const uint32_t w = BF::pack(w0, w1);
-            if constexpr (SPLIT) wl[nt][r] = transpose8(BF::pack(w0 - BF::lo(w), w1 - BF::hi(w)));
+            wl[nt][r] = transpose8(BF::pack(w0 - BF::lo(w), w1 - BF::hi(w)));
             wb[nt][r] = transpose8(w);
           }
         }
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, ctas_of(NT)) attend_kv4_mma
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma<__nv_bfloat16>(o[blk * 2 + k][nt], f, wb[nt][0], wb[nt][1]);
-            if constexpr (SPLIT) mma<__nv_bfloat16>(o[blk * 2 + k][nt], f, wl[nt][0], wl[nt][1]);
+            mma<__nv_bfloat16>(o[blk * 2 + k][nt], f, wl[nt][0], wl[nt][1]);
           }
         }
       }

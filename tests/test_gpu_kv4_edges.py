@@ -74,3 +74,16 @@ def test_weights_of_the_windows_keep_their_bits(cuda, dtype, Dh, seed):
     st = _state(g, 1, 1, 1, Dh, dtype, 64, 16, 0, 0, [4 + seed], 1, 0, cuda)
     _cancel(st, 4 + seed)
     _check_weights(_run(st, cuda), st)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Dh", [64, 128, 256])
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_weights_of_the_record_keep_their_bits(cuda, dtype, Dh, seed):
+    """An opened group against an exact row that cancels it."""
+    g = torch.Generator().manual_seed(100 + seed)
+    st = _state(g, 1, 1, 1, Dh, dtype, 64, 16, 0, 0, [64 + seed], 1, 1, cuda)
+    assert (st["gid"] >= 0).all()
+    st["q"] *= 0.25            # many keys count
+    _cancel(st, seed)
+    _check_weights(_run(st, cuda), st)
