@@ -1,7 +1,8 @@
 """Linear layers with 8-bit block-scaled weights, the format of FP8 checkpoints: e4m3 values [N, K] and one fp32
 scale per 128 x 128 block, activations quantised per token and 128 channels in the layer
 (``ops.fp8_linear``).  The attributes carry the checkpoints' names (``weight``, ``weight_scale_inv``,
-``bias``), so such a state_dict loads unchanged.  Inference only.
+``bias``), so such a state_dict loads unchanged; weight and scales keep their types when a model is moved to
+another one.  Inference only.
 
 No counterpart in the reference, which calls the model library's own FP8 layers (its patch is "FP8-safe" by
 reusing them by reference, qwen_routed_attention.py:94-156).
@@ -36,6 +37,20 @@ class Fp8Linear(nn.Module):
         if lin.bias is not None:
             m.bias = lin.bias.detach().clone()
         return m
+
+    def _apply(self, fn, recurse: bool = True):
+        # moves of a model reach its layers through here: devices apply to the weight and its scales, a type
+        # (model.bfloat16(), .half(), .to(dtype)) to the bias alone
+        held = (self.weight, self.weight_scale_inv)
+
+        def keep(t: torch.Tensor) -> torch.Tensor:
+            if any(t is h for h in held):
+                probe = fn(t.new_empty(0))
+                if probe.dtype != t.dtype:
+                    return t.to(probe.device)
+            return fn(t)
+
+        return super()._apply(keep, recurse)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return ops.fp8_linear(x, self.weight, self.weight_scale_inv, bias=self.bias)
