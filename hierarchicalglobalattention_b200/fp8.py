@@ -66,13 +66,14 @@ def fp8_weight_of(m: nn.Module) -> Optional[Tuple[torch.Tensor, torch.Tensor, Op
     if tuple(s.shape) != (-(-w.shape[0] // blk), -(-w.shape[1] // blk)):
         return None
     bias = getattr(m, "bias", None)
-    return w.detach(), s.detach().float().contiguous(), None if bias is None else bias.detach()
+    return w.detach().contiguous(), s.detach().float().contiguous(), None if bias is None else bias.detach().contiguous()
 
 
 def fp8_concat(mods: Sequence[nn.Module]) -> Optional[Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]]:
     """One (weight, scales, bias) for layers that share their input, so that they run as one product: 8-bit
     layers as they are, plain ``nn.Linear`` layers quantised.  None when a layer is neither, or when a layer but
-    the last ends inside a 128-feature block (its scales would not line up)."""
+    the last ends inside a 128-feature block (its scales would not line up).  A single 8-bit layer's tensors
+    come as they are, without a copy."""
     parts = []
     for i, m in enumerate(mods):
         p = fp8_weight_of(m)
@@ -83,6 +84,8 @@ def fp8_concat(mods: Sequence[nn.Module]) -> Optional[Tuple[torch.Tensor, torch.
         parts.append(p)
     if len({p[0].shape[1] for p in parts}) != 1:
         raise _lib.HgaError("fp8_concat: the layers differ in their input's width")
+    if len(parts) == 1:
+        return parts[0]
     bias = None
     if any(p[2] is not None for p in parts):
         dt = next(p[2].dtype for p in parts if p[2] is not None)

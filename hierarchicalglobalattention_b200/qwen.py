@@ -23,7 +23,8 @@ key by DCA chunk).
 Low-bit layers (no counterpart in the reference): ``kv_bits=4`` keeps the cold token record in 4 bits
 (``Kv4CacheStore``: in HBM for cache_location "vram", in pinned host memory for "ram"), and
 ``fp8_projections=True`` runs the q/k/v and output projections as 8-bit block-scaled products - the layers of
-an FP8 checkpoint as they are, plain linear layers quantised once.  Not carried over: the file-system cache tier (``cache_location="fs"``), which
+an FP8 checkpoint without a conversion (o_proj where it is, q/k/v copied side by side like the 16-bit ones), plain linear
+layers quantised once.  Not carried over: the file-system cache tier (``cache_location="fs"``), which
 raises.
 """
 from __future__ import annotations
@@ -36,7 +37,7 @@ import torch.nn.functional as F
 
 from .config import ChunkPlacementPolicy, RouterConfig
 from . import ops
-from .fp8 import fp8_concat
+from .fp8 import fp8_concat, fp8_weight_of
 from .module import routed_attention
 from .router import ChunkRouter
 from .store import VramKVCacheStore
@@ -159,8 +160,12 @@ class QwenRoutedAttention(nn.Module):
 
     def _fp8(self, x: torch.Tensor, name: str, mods) -> torch.Tensor:
         """The layers' outputs on x, side by side, as 8-bit block-scaled products: one for all of them when
-        their blocks line up.  Layers of an FP8 checkpoint are used as they are; plain linear layers are
-        quantised once (again when a weight changes)."""
+        their blocks line up.  A single layer of an FP8 checkpoint is used where it is; several are copied side by
+        side into one weight, plain linear layers are quantised, once (again when a weight changes)."""
+        own = fp8_weight_of(mods[0]) if len(mods) == 1 else None
+        if own is not None:
+            w, s, b = own
+            return ops.fp8_linear(x, w, s, bias=None if b is None else b.to(x.dtype))
         ts = tuple(m.weight for m in mods) + tuple(getattr(m, "weight_scale_inv", None) for m in mods) + tuple(
             getattr(m, "bias", None) for m in mods)
         hit = self._fp8_cache.get(name)

@@ -36,3 +36,27 @@ def test_meta_and_empty_moves():
     n = _model()
     m.load_state_dict(n.state_dict())
     assert torch.equal(m[0].weight.float(), n[0].weight.float())
+
+
+def test_a_single_8bit_layer_is_used_where_it_is(monkeypatch):
+    """o_proj of an FP8 checkpoint: the product reads the layer's own tensors and the wrapper keeps no copy."""
+    import types
+    import hierarchicalglobalattention_b200 as hga
+    from hierarchicalglobalattention_b200 import ops
+    from hierarchicalglobalattention_b200.fp8 import fp8_concat
+    torch.manual_seed(1)
+    o = Fp8Linear.from_linear(nn.Linear(128, 64).bfloat16())
+    w, s, b = fp8_concat([o])
+    assert w.data_ptr() == o.weight.data_ptr() and s.data_ptr() == o.weight_scale_inv.data_ptr()
+    assert b.data_ptr() == o.bias.data_ptr()
+    seen = []
+    monkeypatch.setattr(ops, "fp8_linear", lambda x, w, s, bias=None: seen.append((w, s, bias)) or x)
+    cfg = types.SimpleNamespace(num_attention_heads=2, num_key_value_heads=1, head_dim=64, hidden_size=64)
+    orig = nn.Module()
+    orig.o_proj = o
+    layer = hga.QwenRoutedAttention(orig, cfg, fp8_projections=True)
+    layer._o_proj(torch.zeros(1, 128, dtype=torch.bfloat16))
+    assert seen[-1][0].data_ptr() == o.weight.data_ptr() and not layer._fp8_cache
+    o.weight = torch.zeros(64, 128).to(torch.float8_e4m3fn)      # a replaced weight is seen, the old one let go
+    layer._o_proj(torch.zeros(1, 128, dtype=torch.bfloat16))
+    assert seen[-1][0].data_ptr() == o.weight.data_ptr()
