@@ -382,11 +382,21 @@ def append_tokens(p: HgaParams, seq_pos: torch.Tensor, k_rope: torch.Tensor, v: 
 # ---------------------------------------------------------------------------------------------
 FP8_BLOCK = 128
 _FP8_X = {**_lib.DTYPE_CODE, torch.float8_e4m3fn: _lib.E4M3_CODE}
-
-
-
-
 _FP8_FEW_ROWS = 16
+
+
+class _NoBackward(torch.autograd.Function):
+    """Ties an operator without a backward to the graph of its inputs: forward runs it, backward says that it has
+    none (as the dispatcher operators do) instead of leaving the gradient out."""
+
+    @staticmethod
+    def forward(ctx, what, call, *inputs):
+        ctx.what = what
+        return call()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise _lib.HgaError(f"{ctx.what} has no backward: call it under torch.no_grad() or detach its inputs")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -398,7 +408,9 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [..., K] (fp32 / bf16 / fp16) as e4m3 values [..., K] and fp32 scales [..., ceil(K / 128)], one
-    per row and block of 128 channels (see hga_fp8_quantize)."""
+    per row and block of 128 channels (see hga_fp8_quantize).  Without a backward: one through it raises."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return _NoBackward.apply("fp8_quantize", lambda: fp8_quantize(x), x)
     if not x.is_cuda:
         _require_cuda(x)
     code = _lib.DTYPE_CODE.get(x.dtype)
@@ -442,7 +454,14 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     ceil(K / 128)] (see hga_fp8_linear).  x [..., K]: fp32 / bf16 / fp16 rows are quantised per row and
     128 channels on the way in; e4m3 rows come with ``x_scale`` [..., ceil(K / 128)], as fp8_quantize
     returns them.  The result [..., N] has ``out_dtype``: x's type, or bf16 for 8-bit x.  ``bias`` [N] has
-    the result's type."""
+    the result's type.  Without a backward: one through it raises."""
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or w_scale.requires_grad
+                                    or (bias is not None and bias.requires_grad)
+                                    or (x_scale is not None and x_scale.requires_grad)):
+        if out is not None:
+            raise _lib.HgaError("fp8_linear: out goes with inputs that require no gradient (use torch.no_grad())")
+        return _NoBackward.apply("fp8_linear", lambda: fp8_linear(x, w, w_scale, bias, x_scale, out_dtype), x, w, w_scale,
+                                 bias, x_scale)
     dev, idx = x.device, x.get_device()
     for t in (w, w_scale, bias, x_scale, out):
         if t is not None and t.get_device() != idx:
