@@ -278,7 +278,7 @@ class ChunkRouter:
         self._rot_stage_ready()
         nmax = max(seq_lens) // C
         st = store.ensure_capacity(layer, max(nmax, 1), max(seq_lens) + C)
-        store.write_tokens(layer, 0, k_rope, v)
+        store.seed_tokens(layer, k_rope, v)
         for b, S in enumerate(seq_lens):
             n = S // C
             if n:
@@ -305,7 +305,7 @@ class ChunkRouter:
             ops.summaries(hp, k_raw, k_rope, v, cos32, sin32, seq_len=n_closed * C,
                           out=(st.chunk_k, st.group_k, st.group_v), out_chunk0=0)
         if st.token_k.data_ptr() != k_rope.data_ptr():
-            store.write_tokens(layer, 0, k_rope, v)
+            store.seed_tokens(layer, k_rope, v)
         store.mark_closed(layer, n_closed)
         rem = S - n_closed * C
         self._active_len[layer] = rem

@@ -203,6 +203,10 @@ class VramKVCacheStore(KVCacheStore):
         st.token_k[:, :, row0:row0 + L].copy_(token_k, non_blocking=True)
         st.token_v[:, :, row0:row0 + L].copy_(token_v, non_blocking=True)
 
+    def seed_tokens(self, layer: int, token_k: torch.Tensor, token_v: torch.Tensor) -> None:
+        """Token rows [0, S) of a prefill, which after_seed follows."""
+        self.write_tokens(layer, 0, token_k, token_v)
+
     def seed_closed_chunks(self, layer, chunk_k, group_k, group_v, token_k, token_v) -> None:
         """Bulk ingest of N closed chunks (ram_kv_cache_store.py:483-526).  token_* [B,KVH,N,C,Dh]."""
         N = chunk_k.shape[2]

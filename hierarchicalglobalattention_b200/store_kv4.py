@@ -38,7 +38,7 @@ class Kv4CacheStore(RamKVCacheStore):
             raise ValueError("the 4-bit record needs a group_size that is a multiple of 16 and head_dim 64, 128, 192 or 256")
         self.record_device = record_device
         self.units_per_group = gs // ops.KV4_UNIT
-        # exact rows of a prefill between the packing and the filling of the windows
+        # exact rows of a prefill between seed_tokens and the filling of the windows (after_seed)
         self._seed_rows: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = {}
 
     # -- buffers -----------------------------------------------------------------------------
@@ -86,9 +86,12 @@ class Kv4CacheStore(RamKVCacheStore):
         """Pack rows [row0, row0 + L); row0 a multiple of 16."""
         if row0 % ops.KV4_UNIT:
             raise ValueError("rows enter the 4-bit record in whole 16-token units")
-        if row0 == 0:
-            self._seed_rows[layer] = (token_k, token_v)
         ops.kv4_pack(token_k, token_v, self.record(layer), unit0=row0 // ops.KV4_UNIT)
+
+    def seed_tokens(self, layer: int, token_k: torch.Tensor, token_v: torch.Tensor) -> None:
+        """A prefill's rows: packed, and held until after_seed has filled the windows from them."""
+        self.write_tokens(layer, 0, token_k, token_v)
+        self._seed_rows[layer] = (token_k, token_v)
 
     def on_chunk_closed(self, layer: int, n: int, row: Optional[int] = None) -> None:
         """The completed active chunk is packed into the record and enters its window slots."""
@@ -99,23 +102,31 @@ class Kv4CacheStore(RamKVCacheStore):
         super().on_chunk_closed(layer, n, row)
 
     def after_seed(self, layer: int, seq_len: int, row: Optional[int] = None) -> None:
-        """Fill the window / active slots from the prefill's exact rows (RamKVCacheStore.after_seed reads them
-        back from its record)."""
-        k, v = self._seed_rows[layer]
+        """Fill the window / active slots: from the prefill's exact rows where seed_tokens brought them, else with
+        the record's values (RamKVCacheStore.after_seed reads its record)."""
+        seed = self._seed_rows.get(layer)
         C, n = self.C, seq_len // self.C
         f_lo, f_hi = self.policy.hot_first_range(n)
         l_lo, l_hi = self.policy.hot_last_range(n)
         bs = slice(None) if row is None else slice(row, row + 1)
+
+        def rows(r0: int, r1: int) -> Tuple[torch.Tensor, torch.Tensor]:
+            if seed is not None:
+                return seed[0][bs, :, r0:r1], seed[1][bs, :, r0:r1]
+            self._sync_record()
+            u0, u1 = r0 // ops.KV4_UNIT, -(-r1 // ops.KV4_UNIT)
+            return self._unpacked(tuple(t[bs, :, u0:u1] for t in self.record(layer)), r1 - r0)
+
         for c in sorted(set(range(f_lo, f_hi)) | set(range(l_lo, l_hi))):
-            sl = slice(c * C, (c + 1) * C)
-            self._to_slot(layer, c, k[bs, :, sl], v[bs, :, sl], None if row is None else 0, row)
+            self._to_slot(layer, c, *rows(c * C, (c + 1) * C), None if row is None else 0, row)
         rem = seq_len - n * C
         if rem:
             k_act, v_act = self.active_rows(layer, n)
-            k_act[bs, :, :rem].copy_(k[bs, :, n * C:seq_len])
-            v_act[bs, :, :rem].copy_(v[bs, :, n * C:seq_len])
+            k, v = rows(n * C, seq_len)
+            k_act[bs, :, :rem].copy_(k)
+            v_act[bs, :, :rem].copy_(v)
         if row is None or row == self.B - 1:
-            del self._seed_rows[layer]
+            self._seed_rows.pop(layer, None)
 
     # -- the VRAM bank, on packed groups ---------------------------------------------------------
     def _group_bytes(self) -> int:
