@@ -116,7 +116,7 @@ def attend_decode(pi: List[int], pf: List[float], q: Tensor, seq_pos: Tensor, ho
 
 @attend_decode.register_fake
 def _(pi, pf, q, seq_pos, hot_k, hot_v, hot_mode, cold_k, cold_v, open_gid, open_t0):
-    return torch.empty_like(q)
+    return q.new_empty(q.shape)
 
 
 @torch.library.custom_op("hga::attend_decode_dca", mutates_args=())
@@ -131,7 +131,7 @@ def attend_decode_dca(pi: List[int], pf: List[float], q: Tensor, seq_pos: Tensor
 @attend_decode_dca.register_fake
 def _(pi, pf, q, seq_pos, hot_k, hot_v, hot_mode, cold_k, cold_v, open_gid, open_t0, open_pos, dca_chunk, dca_ceil,
       theta):
-    return torch.empty_like(q)
+    return q.new_empty(q.shape)
 
 
 @torch.library.custom_op("hga::gather_h2d", mutates_args=("bank_k", "bank_v", "slot_gid", "gid_slot", "slot_stamp",
@@ -145,7 +145,7 @@ def gather_h2d(pi: List[int], pf: List[float], open_gid: Tensor, rec_k: Tensor, 
 
 @gather_h2d.register_fake
 def _(pi, pf, open_gid, rec_k, rec_v, bank_k, bank_v, slot_gid, gid_slot, slot_stamp, stamp, counters):
-    return torch.empty_like(open_gid)
+    return open_gid.new_empty(open_gid.shape)
 
 
 # ---- 8-bit products and the 4-bit record ------------------------------------------------------
@@ -204,4 +204,4 @@ def attend_decode_kv4(pi: List[int], pf: List[float], q: Tensor, seq_pos: Tensor
 
 @attend_decode_kv4.register_fake
 def _(pi, pf, q, seq_pos, hot_k, hot_v, rec_k, rec_v, open_gid, open_t0):
-    return torch.empty_like(q)
+    return q.new_empty(q.shape)
