@@ -16,6 +16,9 @@ from ._lib import HgaParams, check, lib, ptr, stream_ptr
 
 Q_BHSD, Q_BSHD = 0, 1
 
+# The device that a launch goes to; an operator whose tensors are on another one switches to it for its call.
+_current_device = torch._C._cuda_getDevice
+
 
 def _require_cuda(*ts):
     for t in ts:
@@ -413,6 +416,9 @@ def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         return _NoBackward.apply("fp8_quantize", lambda: fp8_quantize(x), x)
     if not x.is_cuda:
         _require_cuda(x)
+    if x.get_device() != _current_device():
+        with torch.cuda.device(x.get_device()):
+            return fp8_quantize(x)
     code = _lib.DTYPE_CODE.get(x.dtype)
     shape = x.shape
     if code is None or not shape or shape[-1] == 0:
@@ -469,6 +475,9 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
             raise _lib.HgaError("fp8_linear: tensors on different devices")
     if idx < 0:
         _require_cuda(x)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return fp8_linear(x, w, w_scale, bias, x_scale, out_dtype, out)
     code = _FP8_X.get(x.dtype)
     if code is None:
         raise _lib.HgaError(f"fp8_linear: x must be fp32, bf16, fp16 or e4m3; got {x.dtype}")
@@ -576,6 +585,9 @@ def kv4_pack(k: torch.Tensor, v: torch.Tensor, rec: Optional[Tuple[torch.Tensor,
     idx = k.get_device()
     if v.get_device() != idx:
         raise _lib.HgaError("kv4_pack: tensors on different devices")
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return kv4_pack(k, v, rec, unit0)
     units = -(-S // KV4_UNIT)
     if rec is None:
         cap = unit0 + units
@@ -613,6 +625,9 @@ def kv4_unpack(rec_k: torch.Tensor, rec_v: torch.Tensor, seq_len: int, dtype: to
         raise _lib.HgaError("hga ops run on CUDA tensors only (no CPU fallback): give kv4_unpack a CUDA device")
     if dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return kv4_unpack(rec_k, rec_v, seq_len, dtype, unit0, dev)
     cap = _kv4_rec("kv4_unpack", rec_k, B, KVH, Dh, dev.index)
     if _kv4_rec("kv4_unpack", rec_v, B, KVH, Dh, dev.index) != cap:
         raise _lib.HgaError("kv4_unpack: rec_k and rec_v differ in capacity")
@@ -635,6 +650,9 @@ def attend_decode_kv4(p: HgaParams, q: torch.Tensor, seq_pos: torch.Tensor, hot_
         if t.get_device() != idx or idx < 0:
             _require_cuda(q, seq_pos, hot_k, hot_v, open_gid, open_t0)
             raise _lib.HgaError("attend_decode_kv4: tensors on different devices")
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return attend_decode_kv4(p, q, seq_pos, hot_k, hot_v, rec_k, rec_v, open_gid, open_t0, out)
     if not q.is_contiguous():
         q = q.contiguous()
     B, H, L, Dh = q.shape
