@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libhga_b200.so")
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 E4M3_CODE = 3    # torch.float8_e4m3fn, the 8-bit operands of hga_fp8_linear
+E_WORKSPACE = -5  # HGA_E_WORKSPACE: nothing was launched, the call needs a workspace
 
 _lib = None
 _lock = threading.Lock()

@@ -496,7 +496,8 @@ int hga_fp8_linear(int64_t m, int64_t n, int64_t k, int32_t x_dtype, const void*
   const hga::Fp8Linear a{m, n, k, x, x_stride, x_dtype, x_scale, w, w_stride, w_scale, ws_stride, bias, out, out_stride,
                          out_dtype, workspace};
   const int64_t need = hga::fp8_linear_workspace(a);
-  if (need > workspace_bytes || (need && (!workspace || ((uintptr_t)workspace & 15))))
+  if (need && !workspace) return fail(HGA_E_WORKSPACE, "hga_fp8_linear: needs a workspace (hga_fp8_linear_workspace)");
+  if (need > workspace_bytes || (need && ((uintptr_t)workspace & 15)))
     return fail(HGA_E_INVALID, "hga_fp8_linear: needs %lld bytes of 16-byte aligned workspace", (long long)need);
   return cuda_status(hga::launch_fp8_linear(a, stream), "hga_fp8_linear");
 }

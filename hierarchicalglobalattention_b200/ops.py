@@ -521,9 +521,13 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     call = (M, N, K, code, xp, xst, None if xs is None else xs.data_ptr(), wp, wst, w_scale.data_ptr(), sst,
             None if bias is None else bias.data_ptr(), ocode, out.data_ptr(), N)
     stream = stream_ptr(dev)
-    # few rows mostly need no workspace: asked for only when the call says so
-    if M <= _FP8_FEW_ROWS and h.hga_fp8_linear(*call, None, 0, stream) == 0:
-        return out
+    if M <= _FP8_FEW_ROWS:
+        # few rows mostly need no workspace: asked for only when the call says so
+        rc = h.hga_fp8_linear(*call, None, 0, stream)
+        if rc == 0:
+            return out
+        if rc != _lib.E_WORKSPACE:
+            check(rc, "hga_fp8_linear")
     need = h.hga_fp8_linear_workspace(M, N, K, code, xp, xst, wp, wst)
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     rc = h.hga_fp8_linear(*call, None if ws is None else ws.data_ptr(), need, stream)

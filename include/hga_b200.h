@@ -32,7 +32,8 @@ enum { HGA_DTYPE_F32 = 0, HGA_DTYPE_BF16 = 1, HGA_DTYPE_F16 = 2,
 enum { HGA_ROT_F32 = 0,         /* fp32 table, used as fp32 (ChunkRouter._rotary_for_positions) */
        HGA_ROT_MODEL = 1,       /* table already in the model dtype */
        HGA_ROT_F32_ROUNDED = 2  /* fp32 table, each entry rounded to the model dtype first (cos.to(x.dtype)) */ };
-enum { HGA_OK = 0, HGA_E_INVALID = -1, HGA_E_UNSUPPORTED = -2, HGA_E_CUDA = -3, HGA_E_DEVICE = -4 };
+enum { HGA_OK = 0, HGA_E_INVALID = -1, HGA_E_UNSUPPORTED = -2, HGA_E_CUDA = -3, HGA_E_DEVICE = -4,
+       HGA_E_WORKSPACE = -5 /* nothing launched: call again with a workspace */ };
 
 /* Hyper-parameters of one routed-attention layer.  Mirrors RouterConfig + ChunkPlacementPolicy
  * (ExistingModelFineTuning/KvRouter/chunk_router.py:59-90, chunk_placement_policy.py:13-38). */
@@ -270,7 +271,8 @@ int hga_fp8_quantize(int64_t m, int64_t k, int32_t dtype, const void* x, int64_t
  * [m][ceil(k / 128)] are used as they are (x_scale is ignored otherwise).  Products and sums in fp32,
  * one rounding to out_dtype (F32 / BF16 / F16) at the end; bias [n] in out_dtype, or NULL.  x_stride and
  * out_stride in elements, any value >= the row.  The call needs hga_fp8_linear_workspace(...) bytes of
- * 16-byte aligned device memory, which it may overwrite (0 bytes: workspace may be NULL). */
+ * 16-byte aligned device memory, which it may overwrite (0 bytes: workspace may be NULL).  With a NULL workspace
+ * where one is needed it returns HGA_E_WORKSPACE: a caller may ask so, as few rows mostly need none. */
 int64_t hga_fp8_linear_workspace(int64_t m, int64_t n, int64_t k, int32_t x_dtype, const void* x, int64_t x_stride,
                                  const void* w, int64_t w_stride);
 int hga_fp8_linear(int64_t m, int64_t n, int64_t k, int32_t x_dtype, const void* x, int64_t x_stride,

@@ -63,3 +63,43 @@ def test_launches_go_to_the_tensors_device(recorded, at):
     names = {n for n, _ in h.calls}
     assert {"hga_fp8_quantize", "hga_fp8_linear", "hga_kv4_pack", "hga_kv4_unpack", "hga_attend_decode_kv4"} <= names
     assert {d for _, d in h.calls} == {at} and state["device"] == 0
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+@pytest.mark.parametrize("codes,want", [([0], 1), ([_lib.E_WORKSPACE, 0], 2), ([-3], 1), ([_lib.E_WORKSPACE, -3], 2)])
+def test_only_a_missing_workspace_is_asked_for_again(recorded, monkeypatch, codes, want):
+    """A product of few rows is first called without a workspace; any other error is raised as it is, once."""
+    calls = []
+
+    class Library:
+        def hga_fp8_linear(self, *a):
+            calls.append(a[15:17])
+            return codes[len(calls) - 1]
+
+        def hga_fp8_linear_workspace(self, *a):
+            return 1024
+
+        def hga_last_error(self):
+            return b"text of the library"
+
+    monkeypatch.setattr(ops, "lib", Library)
+    monkeypatch.setattr(_lib, "lib", Library)
+    with FakeTensorMode():
+        x = torch.empty(3, 256, device="cuda:0", dtype=torch.bfloat16)
+        w = torch.empty(128, 256, device="cuda:0", dtype=torch.float8_e4m3fn)
+        ws = torch.empty(1, 2, device="cuda:0")
+        if codes[-1]:
+            with pytest.raises(_lib.HgaError, match="text of the library"):
+                ops.fp8_linear(x, w, ws)
+        else:
+            ops.fp8_linear(x, w, ws)
+    assert len(calls) == want and calls[0] == (None, 0)
+
+
+def test_a_missing_workspace_has_its_own_code():
+    import ctypes
+    one = ctypes.c_void_p(16)
+    h = _lib.lib()
+    args = (4000, 4096, 4096, 1, one, 4096, None, one, 4096, one, 32, None, 1, one, 4096)
+    assert h.hga_fp8_linear(*args, None, 0, None) == _lib.E_WORKSPACE and b"workspace" in h.hga_last_error()
+    assert h.hga_fp8_linear(*args, one, 16, None) == -1
