@@ -481,14 +481,14 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     code = _FP8_X.get(x.dtype)
     if code is None:
         raise _lib.HgaError(f"fp8_linear: x must be fp32, bf16, fp16 or e4m3; got {x.dtype}")
-    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.stride(1) != 1:
+    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or (w.stride(1) != 1 and w.shape[1] > 1):
         raise _lib.HgaError("fp8_linear: w must be an e4m3 [N, K] tensor with contiguous rows")
     N, K = w.shape
     KB, NB = -(-K // FP8_BLOCK), -(-N // FP8_BLOCK)
     shape = x.shape
     if not shape or shape[-1] != K or K == 0 or N == 0:
         raise _lib.HgaError(f"fp8_linear: x {tuple(shape)} does not fit w {tuple(w.shape)}")
-    if w_scale.dtype != torch.float32 or w_scale.shape != (NB, KB) or w_scale.stride(1) != 1:
+    if w_scale.dtype != torch.float32 or w_scale.shape != (NB, KB) or (w_scale.stride(1) != 1 and KB > 1):
         raise _lib.HgaError(f"fp8_linear: w_scale must be fp32 [{NB}, {KB}] with contiguous rows")
     xs = None
     if code == _lib.E4M3_CODE:

@@ -103,3 +103,20 @@ def test_a_missing_workspace_has_its_own_code():
     args = (4000, 4096, 4096, 1, one, 4096, None, one, 4096, one, 32, None, 1, one, 4096)
     assert h.hga_fp8_linear(*args, None, 0, None) == _lib.E_WORKSPACE and b"workspace" in h.hga_last_error()
     assert h.hga_fp8_linear(*args, one, 16, None) == -1
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+def test_strides_of_dimensions_of_size_one_are_free(recorded):
+    """One block of channels, or one channel: a transposed row is a column as good as any."""
+    h, _ = recorded
+    with FakeTensorMode():
+        for K in (1, 100):
+            x = torch.empty(40, K, device="cuda:0", dtype=torch.bfloat16)
+            w = torch.empty(K, 300, device="cuda:0", dtype=torch.float8_e4m3fn).t()
+            w = w if K == 1 else torch.empty(300, K, device="cuda:0", dtype=torch.float8_e4m3fn)
+            ws = torch.empty(1, 3, device="cuda:0").t()
+            assert ws.stride(1) != 1
+            assert ops.fp8_linear(x, w, ws).shape == (40, 300)
+        with pytest.raises(_lib.HgaError, match="w_scale"):
+            ops.fp8_linear(torch.empty(4, 200, device="cuda:0"), torch.empty(300, 200, device="cuda:0", dtype=w.dtype),
+                           torch.empty(2, 3, device="cuda:0").t())
