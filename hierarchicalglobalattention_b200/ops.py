@@ -657,8 +657,8 @@ def attend_decode_kv4(p: HgaParams, q: torch.Tensor, seq_pos: torch.Tensor, hot_
     if idx != _current_device():
         with torch.cuda.device(idx):
             return attend_decode_kv4(p, q, seq_pos, hot_k, hot_v, rec_k, rec_v, open_gid, open_t0, out)
-    if not q.is_contiguous():
-        q = q.contiguous()
+    if not q.is_contiguous() or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
     B, H, L, Dh = q.shape
     dtype = q.dtype
     if B != p.batch or H != p.nhead or Dh != p.head_dim or _lib.DTYPE_CODE.get(dtype) != p.dtype:

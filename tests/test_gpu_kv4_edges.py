@@ -87,3 +87,17 @@ def test_weights_of_the_record_keep_their_bits(cuda, dtype, Dh, seed):
     st["q"] *= 0.25            # many keys count
     _cancel(st, seed)
     _check_weights(_run(st, cuda), st)
+
+
+def test_queries_off_the_16_byte_grid(cuda):
+    from hierarchicalglobalattention_b200 import ops
+    g = torch.Generator().manual_seed(41)
+    st = _state(g, 2, 8, 2, 128, torch.bfloat16, 64, 16, 1, 1, [700, 300], 3, 8, cuda)
+    want = _run(st, cuda)
+    flat = torch.zeros(st["q"].numel() + 8, dtype=torch.bfloat16, device=cuda)
+    for off in (1, 3, 8):
+        q = flat[off:off + st["q"].numel()].view(st["q"].shape)
+        q.copy_(st["q"])
+        out = ops.attend_decode_kv4(st["p"], q, st["pos"].to(cuda), st["hk"].to(cuda), st["hv"].to(cuda), *st["rec"],
+                                    st["gid"].to(cuda), st["t0"].to(cuda))
+        assert torch.equal(out, want)
