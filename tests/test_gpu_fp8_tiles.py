@@ -8,8 +8,10 @@ from test_gpu_fp8 import _check, _weight, _x
 
 pytestmark = pytest.mark.gpu
 
-# M, N, K: single-CTA 128 x 128 tiles, 256 to 512 of them on 148 SMs; pairs with 64 or fewer columns in the last tile
-SHAPES = [(2048, 2048, 64), (2048, 2048, 128), (1024, 4096, 256), (512, 5120, 128), (4096, 2048 + 64, 128),
+# M, N, K: about 290 tiles of 128 x 128 on 148 SMs, whole and ragged; as many of 256 x 256 as there are CTA pairs, and
+# more; pairs with 64 or fewer columns in the last tile
+SHAPES = [(2432, 1920, 64), (2432, 1920, 128), (2432, 1920, 256), (2432, 1904, 128), (2304 + 9, 1920, 64),
+          (2048, 2048, 64), (2048, 2048, 128), (1024, 4096, 256), (512, 5120, 128), (4096, 2048 + 64, 128),
           (10240, 320, 64), (10240, 320, 256), (20480, 264, 128)]
 
 
