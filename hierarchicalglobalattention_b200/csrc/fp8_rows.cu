@@ -9,10 +9,10 @@
 //              weight is on its way (each slice is small and comes from L2)
 //   warps 2-5  then one feature a thread: sum[token] += D * (ws * xs[token]) per block
 // FUSED saves the quantisation's launch and its round trip through memory; past some 64 blocks a CTA its
-// repetition in every CTA costs more than that (16 x 8192 into 8192 features: 22.3 us against 14.2).
+// repetition in every CTA costs more than that (16 x 8192 into 8192 features: 27.2 us against 19.7).
 // One token of 2048 channels into 5120 features: 7.6 us (the launch of a cluster and the chain of loads, product
 // and join bound it; the weight alone is 1.6 us of HBM); 16 rows of 8192 channels, already quantised, into 8192
-// features: 11.8 us, 5.7 TB/s of weight.
+// features: 16.7 us with the weight in HBM (4.0 TB/s), 11.9 with it in L2.
 #include <cooperative_groups.h>
 
 #include "fp8_common.cuh"
@@ -373,7 +373,10 @@ bool fp8_rows_better(const Fp8Linear& a) {
   return rows_fit(a) && (a.m <= 64 || (a.n + 127) / 128 * ((a.m + tn - 1) / tn) <= 64);
 }
 
-// Quantising inside pays as long as a CTA has no more than about 64 (row, block) pairs of its own.
+// Quantising inside pays as long as a CTA has no more than about 64 (row, block) pairs of its own.  Inside against
+// apart: 1 x 2048 -> 5120 (4 pairs) 7.8 and 8.8 us, 8 x 4096 -> 2048 (32) 8.3 and 9.4, 4 x 8192 -> 8192 (64) 18.5 and
+// 19.2, 16 x 2048 -> 5120 (64) 9.7 and 9.6, 16 x 8192 -> 1024 (128) 11.9 and 10.2, 8 x 8192 -> 8192 (128) 21.3 and 19.3,
+// 16 x 8192 -> 8192 (256) 27.2 and 19.7.
 bool fp8_rows_fused(const Fp8Linear& a) {
   if (a.x_dtype == HGA_DTYPE_E4M3 || a.m > 16 || !rows_fit(a)) return false;
   const int64_t kb = (a.k + 127) / 128, splits = tc::rows_splits(a.m, a.n, kb, 16);

@@ -13,15 +13,15 @@
 //   warp 1      MMA issuer (of the even CTA), TMEM owner
 //   warps 4-11  each reads 32 TMEM lanes (rows) x BN / 2 columns: one row a thread, one weight block a
 //               warp, so a block's scale is one product per thread
-// What bounds it: the loop that a TMEM buffer turns in (MMAs, commit, epilogue, release, next MMAs; two buffers of
-// 256 columns are all of TMEM).  32768 x 2048 into 5120 features: 335 us, 2.05 PFLOP/s in a burst; the MMAs of a
-// 256 x 256 x 128 block take 512 cycles of about 1100.  With the epilogue's reads and sums left out the tiles still
-// took 290 us; three stages of loads instead of five, or every load from the same tile, changed nothing.
+// 32768 x 2048 into 5120 features: 335 us, 2.05 PFLOP/s in a burst, the tensor pipe busy 49 % of the time.  A block
+// of a 256 x 256 tile takes about 1100 cycles, its MMAs 512 of them; what the rest is spent on is not known.  It is
+// not the loads (three stages instead of five, or every load from the same tile, changed nothing), mostly not the
+// epilogue's reads and sums (290 us with them left out), and not a hand-over latency that more buffers would hide:
+// 256 x 128 tiles in four TMEM buffers took 570 us, about 1000 cycles for half the block.
 // Measured and not kept: one CTA on 128 x 256 tiles (48 KB of loads a block) 470 us, sixteen epilogue warps of 64
 // columns 370 (440 with scales ahead, which spill; 395 with two more warps bringing the scales into shared
-// memory), reads 32 columns ahead of the sums 400, 256 x 128 tiles in four TMEM buffers 570, a block's two halves
-// of 128 features as MMAs and hand-overs of their own 375, arrivals with cluster-scope release 690 (a memory
-// barrier each).
+// memory), reads 32 columns ahead of the sums 400, a block's two halves of 128 features as MMAs and hand-overs of
+// their own 375, arrivals with cluster-scope release 690 (a memory barrier each).
 // Results go through two 4 KB pieces of swizzled shared memory per warp to whole-line TMA stores (plain stores where
 // the output's rows are off the 16-byte grid).  Waits are bounded as in tc_common.cuh.
 #include "fp8_common.cuh"

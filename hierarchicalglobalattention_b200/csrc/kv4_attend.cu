@@ -23,10 +23,11 @@
 // then the union); every warp keeps its own online softmax and copies its next units with cp.async (plain
 // loads for records in pinned host memory, where asynchronous copies are slower).  Warps join in shared
 // memory, CTAs through distributed shared memory, in a fixed order: no atomics on results, one launch.
-// One token for each of 16 sequences of 32768 (32 heads over 4): 28 us for 63 MB (2.25 TB/s); issue of the
-// decoding bounds it there (some 400 instructions a unit and warp, 39 % of the SMs' issue), set-up and the two
-// cluster barriers (9 us together) for one sequence: 10.6 us at 4096 tokens.  One pass over keys per query head
-// with plain FMAs took 566 and 398 us.
+// One token for each of 16 sequences of 32768 (32 heads over 4): 28 us for 63 MB (2.25 TB/s).  No single limit is
+// near: 24 % of DRAM's rate, 40 % of the SMs' issue.  While warps are resident half of the issue slots are empty; the
+// four warps a scheduler has at most wait for fixed latencies, the math pipes, loads and barriers in turn (1.2, 0.8,
+// 0.7 and 0.6 cycles an issued instruction).  One sequence is set-up and the two cluster barriers (9 us together): 10.5 us at
+// 4100 tokens.  One pass over keys per query head with plain FMAs took 566 and 398 us.
 #include <cooperative_groups.h>
 
 #include "fp32x2.cuh"
@@ -863,12 +864,12 @@ cudaError_t launch_attend_kv4_mma(const hga_params& p, int L, const void* q, con
   else (void)cudaGetLastError();
   // Heads of a CTA: as many as fill 8 columns with their rows.  More heads mean a longer union that every tile
   // of columns decodes anew, fewer leave columns empty: 64 rows of one sequence, 64 groups opened by each of 8
-  // heads, take 30 us with one head a CTA and 79 with 8 where the heads opened different groups (29 with 8
-  // where all opened the same), 2 rows of each of 16 sequences 44 with 4 and 59 with 8 (21 and 23).
+  // heads, take 32 us with one head a CTA and 92 with 8 where the heads opened different groups (33 and 31
+  // where all opened the same), 2 rows of each of 16 sequences 48 with 4 and 65 with 8 (22 and 24).
   a.hpc = L >= 8 ? 1 : 8 / L;
   if (a.hpc > a.rep) a.hpc = a.rep;
-  // One row of few sequences: half as many heads where twice the CTAs are still resident (4 sequences 13.9
-  // against 17.4 us, or 11.1 and 11.2 with the same groups for all heads).
+  // One row of few sequences: half as many heads where twice the CTAs are still resident (4 sequences 14.3
+  // against 18.4 us, or 11.5 either way with the same groups for all heads).
   if (L == 1 && (int64_t)p.batch * p.kv_heads * ((a.rep + a.hpc - 1) / a.hpc) * 16 <= 132 * kv4::ctas_of(1))
     a.hpc = (a.hpc + 1) / 2;
   const int cols = a.hpc * L;
