@@ -410,9 +410,9 @@ static cudaError_t tiles_t(const Fp8Linear& a, const void* q, int64_t q_stride, 
 template <typename T>
 static cudaError_t tiles_n(const Fp8Linear& a, const void* q, int64_t q_stride, const float* xs, int64_t xs_stride,
                            const void* w, int64_t w_stride, cudaStream_t st) {
-  // 256 x 256 tiles of CTA pairs or 128 x 128 tiles of single CTAs, by the rounds that the GPU's SMs take over them: a
-  // round of pairs (74 tiles) takes about 4/3 of a round of single tiles (148, half the area), 9 against 6.7 us at
-  // 2048 channels.  Measured at 2048 channels, pairs against single: 4096 x 2304 (2 rounds, 4) 23.5 and 32.4 us,
+  // 256 x 256 tiles of CTA pairs or 128 x 128 tiles of single CTAs, by the waves that the GPU's SMs take over them: a
+  // wave of pairs (74 tiles) takes about 4/3 of a wave of single tiles (148, half the area), 9 against 6.7 us at
+  // 2048 channels.  Measured at 2048 channels, pairs against single: 4096 x 2304 (2 waves, 4) 23.5 and 32.4 us,
   // 2304 x 2304 (2, 3) 22.3 and 24.9, 2048 x 2048 (1, 2) 14.0 and 17.9; 2432 x 1920 (2, 2) 22.2 and 18.5, 1408 x 1664
   // (1, 1) 13.3 and 10.7.  At 512 and 8192 channels the order is the same except for 2560 x 2048 x 512 (2, 3), 10.9
   // and 10.3.
